@@ -549,6 +549,127 @@ def paged_decode_attention(q, kv_cache, layer, block_table, seq_lens, out, *, q_
     return out
 
 
+class SharedPrefixPlan:
+    """The work of `shared_prefix_attention` for one set of groups (`shared_prefix_plan`): it depends on the groups
+    and their prefixes alone, so a serving loop keeps it over all layers and steps (and graph replays) until a
+    member is added.  Members that end keep their place with length 0.  Nothing in it changes after it is made."""
+
+    __slots__ = ("items", "groups", "seq_group", "tile_rows", "prefix_splits", "suffix_splits", "batch", "num_q_heads",
+                 "num_kv_heads", "head_dim", "q_len")
+
+
+def _prefix_chunk(prefix: int, per_key_ctas: int, page_multiple: int, slots: int) -> int:
+    """Prefix tokens per split: as many splits as fill `slots` CTAs, each at least one step of the kernel."""
+    if prefix <= 0:
+        return page_multiple
+    steps = -(-prefix // page_multiple)
+    splits = max(1, min(steps, slots // max(1, per_key_ctas)))
+    return -(-steps // splits) * page_multiple
+
+
+def shared_prefix_plan(group_sizes, prefix_lens, *, num_q_heads: int, num_kv_heads: int, head_dim: int, q_len: int = 1,
+                       max_seq_len: Optional[int] = None, device=None) -> SharedPrefixPlan:
+    """Plan for a decode batch whose sequences come in groups: the first group_sizes[0] sequences share their first
+    prefix_lens[0] tokens, and so on (a group of one, or a prefix of 0, is an ordinary sequence).
+
+    max_seq_len bounds the lengths that later calls will see; it only chooses how far a sequence's own pages are
+    split over CTAs (default: the prefix and 1024 tokens more)."""
+    sizes, prefix = [int(n) for n in group_sizes], [int(n) for n in prefix_lens]
+    if len(sizes) != len(prefix):
+        raise ValueError(f"shared_prefix_plan: {len(sizes)} groups but {len(prefix)} prefix lengths")
+    if any(n < 1 for n in sizes) or any(n < 0 for n in prefix):
+        raise ValueError("shared_prefix_plan: groups have at least one sequence and prefixes no negative length")
+    if head_dim not in (64, 128):
+        raise ValueError(f"shared_prefix_plan: head_dim 64 or 128, not {head_dim}")
+    if num_kv_heads < 1 or num_q_heads < 1 or num_q_heads % num_kv_heads:
+        raise ValueError("shared_prefix_plan: q heads must be a multiple of KV heads")
+    if q_len < 1:
+        raise ValueError("shared_prefix_plan: q_len must be at least 1")
+    per_seq = q_len * (num_q_heads // num_kv_heads)  # query rows of a sequence and KV head
+    sms = _num_sms(device.index or 0 if isinstance(device, torch.device) else 0)
+    p = SharedPrefixPlan()
+    rows = [n * per_seq for n in sizes]
+    p.tile_rows = 16 if max(rows, default=0) <= 16 else 32
+    tiles = [-(-r // p.tile_rows) for r in rows]
+    total = sum(t * n for t, n in zip(tiles, prefix)) * num_kv_heads  # row tiles x keys, all groups
+    items, groups, seq_group = [], [], []
+    p.prefix_splits = 1
+    first = 0
+    for g, (n, pre) in enumerate(zip(sizes, prefix)):
+        # every group gets CTAs by its share of the work
+        slots = 4 * sms * tiles[g] * pre * num_kv_heads // max(1, total)
+        chunk = _prefix_chunk(pre, tiles[g] * num_kv_heads, 64, slots)
+        splits = -(-pre // chunk)
+        p.prefix_splits = max(p.prefix_splits, splits)
+        groups.append((first, n, pre, chunk))
+        seq_group += [g] * n
+        items += [(g, t * p.tile_rows, s, 0) for s in range(splits) for t in range(tiles[g])]
+        first += n
+    p.batch, p.num_q_heads, p.num_kv_heads, p.head_dim, p.q_len = first, num_q_heads, num_kv_heads, head_dim, q_len
+    # a sequence's own pages: one CTA per KV head and 32 rows, split while CTAs are few and pages many
+    own = (max_seq_len - min(prefix, default=0)) if max_seq_len is not None else 1024
+    ctas = first * num_kv_heads * (-(-per_seq // 32))
+    p.suffix_splits = 1
+    while p.suffix_splits < 8 and ctas * p.suffix_splits < 2 * sms and own // p.suffix_splits >= 256:
+        p.suffix_splits *= 2
+    p.items = torch.tensor(items, dtype=torch.int32).view(-1, 4).to(device)
+    p.groups = torch.tensor(groups, dtype=torch.int32).view(-1, 4).to(device)
+    p.seq_group = torch.tensor(seq_group, dtype=torch.int32).to(device)
+    return p
+
+
+def shared_prefix_attention(q, kv_cache, layer, block_table, seq_lens, out, *, plan: SharedPrefixPlan, scale: float):
+    """Paged decode / verify attention (q, out [B * q_len, nq, D] bf16, D 64 or 128) of a batch whose groups share
+    prefixes: each prefix is read once for its whole group, and only the rest of a sequence per sequence.
+
+    Same result as `paged_decode_attention` over the same tables: query position i of a sequence sees keys
+    0 .. seq_len - q_len + i.  All members of a group must hold the same K / V for the group's prefix (in the same
+    pages or in copies); it is read through the first member that still holds it.  seq_lens of 0 (padding, ended
+    members) give zeros.  Slots behind a sequence's end may hold anything.  Safe in CUDA graphs: the workspace
+    belongs to the call.  Only bf16 caches (an int8 cache is refused)."""
+    if (q.dim() == 3 and (q.shape[1] != plan.num_q_heads or q.shape[2] != plan.head_dim)) or \
+            (kv_cache.dim() == 6 and kv_cache.shape[3] != plan.num_kv_heads):
+        raise ValueError("shared_prefix_attention: the plan was made for other heads")
+    _C().shared_prefix_attention(q, kv_cache, layer, block_table, seq_lens, out, plan.items, plan.groups,
+                                 plan.seq_group, plan.q_len, plan.tile_rows, plan.prefix_splits, plan.suffix_splits,
+                                 scale)
+    _count(2 if plan.items.shape[0] else 1)
+    return out
+
+
+# ---------------------------------------------------------------- pages shared by sequences
+def kv_fork(kv_cache, block_table, seq_lens, parents, fresh, ref):
+    """Rows for new sequences that continue others: child c takes the pages of block-table row parents[c], whose full
+    pages it shares; a last page that is not full is copied (all layers) to page fresh[c], which must be free.
+
+    kv_cache [L, NB, ...] of any type, contiguous; block_table int32 [S, W]; seq_lens int32 [S]; parents, fresh
+    int32 [C]; ref int32 [NB], the number of rows that hold each page, raised for every page taken.  Returns
+    (table int32 [C, W], lens int32 [C]), entries behind the last page 0.  parents[c] < 0 gives an empty row;
+    fresh[c] is not looked at where the parent's last page is full.  An id out of range, or a fresh page that is
+    not free, sets status bit 8 (`check_status`); such a call's results are not to be used."""
+    r = _C().kv_fork(kv_cache, block_table, seq_lens, parents, fresh, ref)
+    _count()
+    return r
+
+
+def kv_free(block_table, seq_lens, rows, ref) -> None:
+    """Give back the pages of block-table rows `rows` (int32; negative entries are skipped): ref -= 1 on each, and
+    seq_lens[row] = 0, so that freeing a row again does nothing.  Pages whose count reaches 0 are free.  A page that
+    nothing held, or an id out of range, sets status bit 8."""
+    _C().kv_free(block_table, seq_lens, rows, ref)
+    _count()
+
+
+def kv_compact(kv_cache, block_table, seq_lens, ref):
+    """Move the pages with ref > 0 to the front of the cache, in place: with U of them, those at U or above move to
+    the free places below U (both in rising order), in all layers; block_table (entries of seq_lens tokens) and ref
+    follow.  Returns (moved int32 [NB]: a held page's new id, -1 for free ones; used int32 [1] = U), for whoever
+    else keeps page ids.  No host synchronisation.  At most 2^20 pages."""
+    r = _C().kv_compact(kv_cache, block_table, seq_lens, ref)
+    _count(2)
+    return r
+
+
 _PREFILL_TC = os.environ.get("BLOOM_PREFILL_TC", "1") != "0"
 
 
@@ -691,6 +812,23 @@ def sample(logits, temperature, top_p, top_k, seeds, offsets, draft=None, out: O
         _C().sample_rows(logits, temperature, top_p, top_k, seeds, offsets, out)
     else:
         _C().verify_sample_rows(logits, temperature, top_p, top_k, seeds, offsets, draft, out)
+    _count()
+    return out
+
+
+def sample_uniform(logits, u, temperature, top_k=None, top_p=None, min_p=None, out: Optional[torch.Tensor] = None):
+    """Tokens drawn from logits (f32 / bf16 [B, V], V <= 2^18) by given uniforms u (f32 [B], or [B, n] for n draws of
+    a row): int32 of u's shape.
+
+    Weights exp((l - max) / temperature); top_k (int32 [B]) keeps the k largest, ties to the lowest index; top_p
+    (f32 [B]) then keeps, in falling order, every token with less than top_p of the remaining mass ahead of it; min_p
+    (f32 [B]) drops weights below min_p times the largest.  The token is the first kept one, in vocabulary order,
+    whose running sum exceeds u times the kept mass.  temperature <= 0: the largest logit (lowest index).  top_k <= 0,
+    top_p outside (0, 1), min_p <= 0 or an absent tensor: off.  NaN logits count as -inf; a row with nothing to draw
+    from gives -1.  u is taken into [0, 1].  Sums are exact integers: equal inputs give equal tokens."""
+    if out is None:
+        out = torch.empty(u.shape, dtype=torch.int32, device=u.device)
+    _C().sample_uniform(logits, u, temperature, top_k, top_p, min_p, out)
     _count()
     return out
 

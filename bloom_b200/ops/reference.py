@@ -199,3 +199,103 @@ def kv_quantize_int8(x):
 
 def kv_dequantize_int8(q, scale):
     return q.float() * scale.float()[:, None]
+
+
+# ---------------------------------------------------------------- sequences that share a prompt (fp64)
+def paged_attention(q, kv_layer, block_table, seq_lens, q_len: int, scale: float):
+    """(out, magnitude) fp64 [B * q_len, nq, D] of attention over pages kv_layer [NB, 2, KVH, 16, D]: query position i
+    of a sequence sees keys 0 .. seq_len - q_len + i; a row that sees nothing gives 0.  magnitude is the same sum
+    over |v| (for error bounds)."""
+    T, nq, D = q.shape
+    nkv = kv_layer.shape[2]
+    out = torch.zeros(T, nq, D, dtype=torch.float64, device=q.device)
+    mag = torch.zeros_like(out)
+    for b, n in enumerate(seq_lens.tolist()):
+        pages = kv_layer[block_table[b, :(n + 15) // 16].long()].double()
+        kv = pages.permute(1, 2, 0, 3, 4).reshape(2, nkv, -1, D)
+        for i in range(q_len):
+            sees = n - q_len + i + 1
+            if sees <= 0:
+                continue
+            row = q[b * q_len + i].double().view(nkv, nq // nkv, D)
+            p = torch.softmax(row @ kv[0, :, :sees].transpose(1, 2) * scale, -1)
+            out[b * q_len + i] = (p @ kv[1, :, :sees]).reshape(nq, D)
+            mag[b * q_len + i] = (p @ kv[1, :, :sees].abs()).reshape(nq, D)
+    return out, mag
+
+
+def kv_fork(kv_cache, block_table, seq_lens, parents, fresh, ref):
+    """Plain loops of ops.kv_fork (in place on kv_cache and ref)."""
+    table = torch.zeros(len(parents), block_table.shape[1], dtype=torch.int32, device=block_table.device)
+    lens = torch.zeros(len(parents), dtype=torch.int32, device=block_table.device)
+    for c, (p, f) in enumerate(zip(parents.tolist(), fresh.tolist())):
+        if p < 0:
+            continue
+        n = int(seq_lens[p])
+        lens[c] = n
+        for j in range(n // 16):
+            table[c, j] = block_table[p, j]
+            ref[block_table[p, j]] += 1
+        if n % 16:
+            kv_cache[:, f] = kv_cache[:, int(block_table[p, n // 16])]
+            table[c, n // 16] = f
+            ref[f] += 1
+    return table, lens
+
+
+def kv_free(block_table, seq_lens, rows, ref):
+    for r in rows.tolist():
+        if r >= 0:
+            for j in range((int(seq_lens[r]) + 15) // 16):
+                ref[block_table[r, j]] -= 1
+            seq_lens[r] = 0
+
+
+def kv_compact(kv_cache, block_table, seq_lens, ref):
+    held = (ref > 0).tolist()
+    used = sum(held)
+    moved = [p if h else -1 for p, h in enumerate(held)]
+    holes = [p for p in range(used) if not held[p]]
+    for src, dst in zip([p for p in range(used, len(held)) if held[p]], holes):
+        kv_cache[:, dst] = kv_cache[:, src]
+        moved[src] = dst
+        ref[dst] = ref[src]
+        ref[src] = 0
+    for s in range(block_table.shape[0]):
+        for j in range((int(seq_lens[s]) + 15) // 16):
+            block_table[s, j] = moved[int(block_table[s, j])]
+    return (torch.tensor(moved, dtype=torch.int32, device=ref.device),
+            torch.tensor([used], dtype=torch.int32, device=ref.device))
+
+
+def sample_uniform(logits, u, temperature, top_k=None, top_p=None, min_p=None):
+    """Row by row on the host, in fp64 (ops.sample_uniform)."""
+    out = torch.empty(u.shape, dtype=torch.int32)
+    uu = u.cpu().double().view(u.shape[0], u[0].numel() if len(u) else 0)
+    for b in range(logits.shape[0]):
+        x = logits[b].cpu().double()
+        x = torch.where(x.isnan(), float("-inf"), x)
+        best = x.max()
+        at = int((x == best).nonzero()[0])
+        t = float(temperature[b])
+        if best == float("-inf") or not t > 0:
+            out[b] = -1 if best == float("-inf") else at
+            continue
+        w = torch.where(x == best, 1.0, torch.where(x == float("-inf"), 0.0, torch.exp((x - best) / t)))
+        order = torch.sort(x, descending=True, stable=True)[1]
+        k = 0 if top_k is None else int(top_k[b])
+        if k > 0:
+            order = order[:k]
+        p = 1.0 if top_p is None else float(top_p[b])
+        if 0 < p < 1:
+            cum = torch.cumsum(w[order], 0)
+            ahead = torch.cat([torch.zeros(1, dtype=torch.float64), cum[:-1]])
+            order = order[ahead < p * cum[-1]]
+        floor = 0.0 if min_p is None else min(1.0, float(min_p[b]))
+        order = order[(w[order] >= floor) & (w[order] > 0)]
+        ids = order.sort()[0]
+        cum = torch.cumsum(w[ids], 0)
+        for d in range(uu.shape[1]):
+            i = int(torch.searchsorted(cum, uu[b, d] * cum[-1], right=True))
+            out.view(uu.shape)[b, d] = ids[min(i, len(ids) - 1)]
+    return out

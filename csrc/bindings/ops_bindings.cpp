@@ -4,6 +4,7 @@
 
 #include "bloom/ops.h"
 #include "bloom/ops_media.h"
+#include "bloom/ops_share.h"
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "bloom_b200 sm_100a kernels";
@@ -76,9 +77,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("decode_attention_splits", &bloom::decode_attention_splits);
   m.def("decode_head_chunks", &bloom::decode_head_chunks);
   m.def("paged_prefill_attention_tc", &bloom::paged_prefill_attention_tc);
+  m.def("shared_prefix_attention", &bloom::shared_prefix_attention, "decode attention with group-shared prefixes");
+  m.def("kv_fork", &bloom::kv_fork, "block-table rows that share their parent's pages");
+  m.def("kv_free", &bloom::kv_free, "give the pages of table rows back");
+  m.def("kv_compact", &bloom::kv_compact, "move the held pages to the front of the cache");
   m.def("argmax_rows", &bloom::argmax_rows);
   m.def("apply_token_mask", &bloom::apply_token_mask);
   m.def("sample_rows", &bloom::sample_rows);
+  m.def("sample_uniform", &bloom::sample_uniform, "draws from given uniforms");
   m.def("verify_sample_rows", &bloom::verify_sample_rows);
   m.def("qgemv", &bloom::qgemv, py::arg("x"), py::arg("qs"), py::arg("scales"), py::arg("kind"), py::arg("out"),
         py::arg("epi"), py::arg("resid") = py::none());

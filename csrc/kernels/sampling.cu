@@ -18,6 +18,7 @@
 
 #include "bloom/common.cuh"
 #include "bloom/ops.h"
+#include "bloom/ops_share.h"
 
 namespace bloom {
 namespace {
@@ -537,8 +538,21 @@ void verify_sample_rows(const torch::Tensor& logits, const torch::Tensor& temper
   launch_sample(logits, temperature, top_p, top_k, seeds, offsets, draft.data_ptr<int>(), out);
 }
 
+namespace {
+torch::Tensor per_device[64];
+}
+
+int* status_word(int64_t device) {
+  TORCH_CHECK(device >= 0 && device < 64, "status: bad device");
+  if (!per_device[device].defined()) {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    C10_CUDA_CHECK(cudaStreamIsCapturing(at::cuda::getCurrentCUDAStream(), &st));
+    TORCH_CHECK(st == cudaStreamCaptureStatusNone, "call ops.status() once before capturing a CUDA graph");
+  }
+  return status_tensor(device).data_ptr<int>();
+}
+
 torch::Tensor status_tensor(int64_t device) {
-  static torch::Tensor per_device[64];
   TORCH_CHECK(device >= 0 && device < 64, "status: bad device");
   if (!per_device[device].defined()) {
     per_device[device] =
