@@ -558,13 +558,17 @@ class SharedPrefixPlan:
                  "num_kv_heads", "head_dim", "q_len")
 
 
-def _prefix_chunk(prefix: int, per_key_ctas: int, page_multiple: int, slots: int) -> int:
-    """Prefix tokens per split: as many splits as fill `slots` CTAs, each at least one step of the kernel."""
-    if prefix <= 0:
-        return page_multiple
-    steps = -(-prefix // page_multiple)
-    splits = max(1, min(steps, slots // max(1, per_key_ctas)))
-    return -(-steps // splits) * page_multiple
+def _prefix_chunk(prefix, tiles, step: int, slots: int) -> int:
+    """Prefix tokens per split, the same for all groups: of the multiples of `step` the one that ends first when
+    `slots` CTAs run at a time and a CTA takes as long as its steps and two more (start-up, result)."""
+    most = max((-(-n // step) for n in prefix), default=1)
+    best = None
+    for c in range(max(1, -(-most // 64)), most + 1):  # at most 64 splits
+        ctas = sum(t * -(-n // (c * step)) for t, n in zip(tiles, prefix))
+        cost = -(-ctas // slots) * (c + 2)
+        if best is None or cost < best[0]:
+            best = (cost, c)
+    return best[1] * step if best else step
 
 
 def shared_prefix_plan(group_sizes, prefix_lens, *, num_q_heads: int, num_kv_heads: int, head_dim: int, q_len: int = 1,
@@ -589,16 +593,17 @@ def shared_prefix_plan(group_sizes, prefix_lens, *, num_q_heads: int, num_kv_hea
     sms = _num_sms(device.index or 0 if isinstance(device, torch.device) else 0)
     p = SharedPrefixPlan()
     rows = [n * per_seq for n in sizes]
-    p.tile_rows = 16 if max(rows, default=0) <= 16 else 32
+    # Rows of a CTA's tile.  Up to 32 stream past the keys on mma.sync (several CTAs per SM); more go to tcgen05,
+    # in one 128-row tile or in pairs of them.
+    most = max(rows, default=0)
+    p.tile_rows = 16 if most <= 16 else 32 if most <= 32 else 128 if most <= 128 else 256
     tiles = [-(-r // p.tile_rows) for r in rows]
-    total = sum(t * n for t, n in zip(tiles, prefix)) * num_kv_heads  # row tiles x keys, all groups
+    step, slots = (64, 2 * sms) if p.tile_rows <= 32 else (128 if p.tile_rows == 256 else 256, sms)
+    chunk = _prefix_chunk(prefix, [t * num_kv_heads for t in tiles], step, slots)
     items, groups, seq_group = [], [], []
     p.prefix_splits = 1
     first = 0
     for g, (n, pre) in enumerate(zip(sizes, prefix)):
-        # every group gets CTAs by its share of the work
-        slots = 4 * sms * tiles[g] * pre * num_kv_heads // max(1, total)
-        chunk = _prefix_chunk(pre, tiles[g] * num_kv_heads, 64, slots)
         splits = -(-pre // chunk)
         p.prefix_splits = max(p.prefix_splits, splits)
         groups.append((first, n, pre, chunk))

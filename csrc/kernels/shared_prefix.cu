@@ -53,6 +53,7 @@ struct Args {
   float* part_o;           // [splits, B * ql, nq, D]
   float2* part_ml;         // [splits, B * ql, nq]
   int B, nq, nkv, ql, NB;
+  int parts;               // partial sums per prefix split: 2 where the two streams of a CTA leave one each
   float scale_log2;
   int* status;
 };
@@ -357,6 +358,401 @@ __global__ void __launch_bounds__(kWarps * 32)
   }
 }
 
+// ---------------------------------------------------------------- prefix on tcgen05
+// Groups with more rows than a streaming CTA holds: S = Q K^T and O += P V on the 5th-generation tensor cores, with
+// 128 rows per softmax warpgroup, one thread per row (no exchange between threads).  A CTA runs two such streams that
+// take turns on the tensor pipe, one stream's softmax under the other's MMAs:
+//   pair   (256-row items)  two row tiles over the same K / V tiles, so each K / V tile serves 256 rows
+//   single (128-row items)  one row tile, the streams take alternate K / V tiles and leave one partial sum each
+// TMEM: S0, S1, O0, O1 of 128 columns; P (bf16, two keys per column) is written over the first half of its S and
+// read from there as the A operand, so it never goes through shared memory.  S(i + 1) of a stream is issued only after
+// its P V(i) has completed, which also makes O safe to rescale when S(i + 1) is seen.  The running max is lazy: O is
+// rescaled only when a row's max grows by more than 2^8.
+// Warps 0-7 softmax and epilogue, warp 8 TMA producer and TMEM owner, warp 9 issues the MMAs of both streams from an
+// event loop over their barriers.
+namespace tc {
+
+constexpr int kRows = 128, kKv = 128;
+constexpr int kThreads = 256 + 64;
+constexpr int kTmemCols = 512;
+constexpr float kLazy = 8.f;  // log2 units
+
+template <int D>
+struct Cfg {
+  static constexpr int kRegion = kKv * 128;       // 64 dims of a K or V tile: 128 token rows of 128 bytes
+  static constexpr int kTile = kKv * D * 2;
+  static constexpr int kQ = kRows * D * 2;
+  static constexpr int kStages = D == 128 ? 2 : 4;  // of the K ring and of the V ring
+  static constexpr int kSmem = 2 * kQ + 2 * kStages * kTile + 256 + 1024;
+};
+
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Orders the use of loaded registers behind the wait for them: an empty statement that reads and writes them.
+__device__ __forceinline__ void pin(float (&v)[16]) {
+  asm volatile(""
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                 "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]));
+}
+// D[tmem] (+)= A[tmem] B[smem desc], A: lane = row, two consecutive bf16 k per 32-bit column
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b_desc), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// V as the B operand, its contiguous dimension being N: 64-element atoms `lbo` bytes apart, 8-key groups 1024 apart.
+__device__ __forceinline__ uint64_t desc_mn(uint32_t smem_addr, uint32_t lbo) {
+  return static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu) | static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16 |
+         static_cast<uint64_t>(1024u >> 4) << 32 | static_cast<uint64_t>(1u) << 46 | static_cast<uint64_t>(2u) << 61;
+}
+
+// grid (items, KV heads)
+template <int D, bool kPair>
+__global__ void __launch_bounds__(kThreads, 1)
+    prefix_tc_kernel(const __grid_constant__ CUtensorMap tm, const Args a) {
+  griddep_launch_dependents();
+  using C = Cfg<D>;
+  constexpr int kStages = C::kStages;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sK = smem + 2 * C::kQ;
+  uint8_t* sV = sK + kStages * C::kTile;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + kStages * C::kTile);
+  uint64_t *fullK = bars, *emptyK = bars + 4, *fullV = bars + 8, *emptyV = bars + 12;
+  uint64_t *s_done = bars + 16, *p_ready = bars + 18, *o_done = bars + 20, *q_ready = bars + 22, *drain = bars + 23;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = warp_id(), lane = lane_id();
+  const int4 it = a.items[blockIdx.x];
+  const Group gr = a.groups[it.x];
+  const int kh = blockIdx.y, G = a.nq / a.nkv;
+  const int2 hold = prefix_holder(a, gr);
+  const int* table = a.table + hold.x * a.table_stride;
+  const int k0 = min(it.z * gr.chunk, hold.y), k1 = min(k0 + gr.chunk, hold.y);  // k0 is a multiple of kKv
+  const int n_kt = (k1 - k0 + kKv - 1) / kKv;
+  const int rows = gr.members * a.ql * G;  // of the whole group
+  const bool two = kPair && rows - it.y > kRows;  // the second row tile holds rows
+  // K / V tiles of stream w, and the i-th of them
+  auto count = [&](int w) { return kPair ? (w == 0 || two ? n_kt : 0) : (n_kt - w + 1) / 2; };
+  auto tile = [&](int w, int i) { return kPair ? i : 2 * i + w; };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&fullK[s], 1);
+      mbar_init(&fullV[s], 1);
+      mbar_init(&emptyK[s], two ? 2 : 1);
+      mbar_init(&emptyV[s], two ? 2 : 1);
+    }
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(&s_done[w], 1);
+      mbar_init(&p_ready[w], 4);
+      mbar_init(&o_done[w], 1);
+    }
+    mbar_init(q_ready, kPair ? 8 : 4);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(tmem_slot, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;  // S_w at 128 w, O_w at 256 + 128 w
+
+  if (warp == 8) {
+    if (lane == 0) {
+      const int n_pages = (k1 + PAGE - 1) / PAGE;
+      auto load = [&](int t, uint8_t* dst, uint64_t* bar, int kv) {
+        int ids[kKv / PAGE];
+#pragma unroll
+        for (int p = 0; p < kKv / PAGE; ++p) {
+          const int page = k0 / PAGE + t * (kKv / PAGE) + p;
+          ids[p] = block_id(a, table, page < n_pages ? page : k0 / PAGE);  // behind the end: any page, it is masked
+        }
+        mbar_arrive_expect_tx(bar, C::kTile);
+#pragma unroll
+        for (int p = 0; p < kKv / PAGE; ++p) {
+          const int row = ((ids[p] * 2 + kv) * a.nkv + kh) * PAGE;
+#pragma unroll
+          for (int r = 0; r < D / 64; ++r) tma_load_2d(dst + r * C::kRegion + p * 2048, &tm, bar, 64 * r, row);
+        }
+      };
+      int nK = 0, nV = 0;
+      bool ok = true;
+      uint64_t t_prog = globaltimer_ns();
+      uint32_t spins = 0;
+      while (ok && (nK < n_kt || nV < n_kt)) {  // the rings advance on their own; V never runs ahead of K
+        bool progressed = false;
+        if (nK < n_kt && mbar_test(&emptyK[nK % kStages], ((nK / kStages) & 1) ^ 1u)) {
+          load(nK, sK + nK % kStages * C::kTile, &fullK[nK % kStages], 0);
+          ++nK;
+          progressed = true;
+        }
+        if (nV < nK && mbar_test(&emptyV[nV % kStages], ((nV / kStages) & 1) ^ 1u)) {
+          load(nV, sV + nV % kStages * C::kTile, &fullV[nV % kStages], 1);
+          ++nV;
+          progressed = true;
+        }
+        if (progressed) {
+          t_prog = globaltimer_ns();
+        } else if ((++spins & 31u) == 0) {
+          if (*abort_flag) {
+            ok = false;
+          } else if (globaltimer_ns() - t_prog > kLocalWaitTimeoutNs) {
+            *abort_flag = 1;
+            atomicOr(a.status, kStatusAttnTimeout);
+            ok = false;
+          }
+        }
+      }
+      if (!ok) {  // the loads in flight land before the block leaves (bounded)
+        for (int j = max(0, nK - kStages); j < nK; ++j) mbar_drain(&fullK[j % kStages], (j / kStages) & 1);
+        for (int j = max(0, nV - kStages); j < nV; ++j) mbar_drain(&fullV[j % kStages], (j / kStages) & 1);
+      }
+    }
+  } else if (warp == 9) {
+    if (lane == 0 && n_kt > 0) {
+      constexpr uint32_t idS = umma_idesc_bf16(kRows, kKv);
+      constexpr uint32_t idO = umma_idesc_bf16(kRows, D) | (1u << 16);  // B is MN-major
+      bool ok = mbar_wait(q_ready, 0, abort_flag, a.status, kStatusAttnTimeout), issued = false;
+      auto issue_s = [&](int w, int t) {
+        tc_fence_after();
+        const int s = t % kStages;
+        const uint32_t kb = smem_u32(sK + s * C::kTile), qb = smem_u32(sQ + (kPair ? w * C::kQ : 0));
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma_f16(tmem + 128 * w, umma_desc_sw128(qb + (kk >> 2) * (kRows * 128)) + 2 * (kk & 3),
+                   umma_desc_sw128(kb + (kk >> 2) * C::kRegion) + 2 * (kk & 3), idS, kk > 0 ? 1u : 0u);
+        umma_commit(&s_done[w]);
+        umma_commit(&emptyK[s]);
+        issued = true;
+      };
+      // per stream: the tile in work, and whether its P V has been issued
+      int i[2] = {0, 0};
+      bool pv[2] = {false, false};
+      int left = 0;
+      for (int w = 0; w < 2 && ok; ++w)
+        if (count(w) > 0) {
+          ++left;
+          const int t = tile(w, 0);
+          ok = mbar_wait(&fullK[t % kStages], (t / kStages) & 1, abort_flag, a.status, kStatusAttnTimeout);
+          if (ok) issue_s(w, t);
+        }
+      uint64_t t_prog = globaltimer_ns();
+      uint32_t spins = 0;
+      while (ok && left > 0) {
+        bool progressed = false;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          if (i[w] >= count(w)) continue;
+          if (!pv[w]) {
+            const int t = tile(w, i[w]), s = t % kStages;
+            if (!mbar_test(&p_ready[w], i[w] & 1) || !mbar_test(&fullV[s], (t / kStages) & 1)) continue;
+            tc_fence_after();
+            const uint32_t vb = smem_u32(sV + s * C::kTile);
+#pragma unroll
+            for (int kk = 0; kk < kKv / 16; ++kk)
+              umma_f16_ts(tmem + 256 + 128 * w, tmem + 128 * w + 8 * kk, desc_mn(vb + kk * 16 * 128, C::kRegion), idO,
+                          (i[w] > 0 || kk > 0) ? 1u : 0u);
+            umma_commit(&o_done[w]);
+            umma_commit(&emptyV[s]);
+            pv[w] = true;
+            if (i[w] + 1 == count(w)) ++i[w], --left;  // the last one: the softmax warps wait for it
+          } else {
+            const int t = tile(w, i[w] + 1);
+            if (!mbar_test(&o_done[w], i[w] & 1) || !mbar_test(&fullK[t % kStages], (t / kStages) & 1)) continue;
+            issue_s(w, t);
+            ++i[w];
+            pv[w] = false;
+          }
+          progressed = true;
+        }
+        if (progressed) {
+          t_prog = globaltimer_ns();
+        } else if ((++spins & 31u) == 0) {
+          if (*abort_flag) {
+            ok = false;
+          } else if (globaltimer_ns() - t_prog > kLocalWaitTimeoutNs) {
+            *abort_flag = 1;
+            atomicOr(a.status, kStatusAttnTimeout);
+            ok = false;
+          }
+        }
+      }
+      if (!ok && issued) {  // what was issued completes before TMEM is freed
+        umma_commit(drain);
+        mbar_drain(drain, 0);
+      }
+    }
+  } else {
+    const int w = warp >> 2, t = threadIdx.x & (kRows - 1);
+    const int r = it.y + (kPair ? w * kRows : 0) + t;
+    const bool valid = r < rows;
+    const bool any = __any_sync(0xffffffffu, valid);
+    const int tok = (valid ? r : 0) / G;
+    const long token = (long)gr.first * a.ql + tok;
+    const int h = kh * G + (valid ? r : 0) % G;
+    if (kPair || w == 0) {  // this thread's q row, K-major with the 128-byte swizzle
+      const uint4* src = reinterpret_cast<const uint4*>(a.q + token * a.q_stride + (long)h * D);
+      uint8_t* dst = sQ + (kPair ? w * C::kQ : 0) + t * 128;
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c)
+        *reinterpret_cast<uint4*>(dst + (c >> 3) * (kRows * 128) + (((c & 7) ^ (t & 7)) << 4)) =
+            valid ? src[c] : make_uint4(0, 0, 0, 0);
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_ready);
+    }
+    const int limit =
+        valid ? min(k1 - 1, seq_len(a, gr.first + tok / a.ql) - a.ql + tok % a.ql) : 0x7fffffff;  // padding: unmasked
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + 128 * w + lanes, tO = tmem + 256 + 128 * w + lanes;
+    float m = kNegBig, l = 0.f;
+    bool failed = false;
+    const int n = count(w);
+    for (int i = 0; i < n; ++i) {
+      if (!mbar_wait(&s_done[w], i & 1, abort_flag, a.status, kStatusAttnTimeout)) failed = true;
+      if (__any_sync(0xffffffffu, failed)) {
+        failed = true;
+        break;
+      }
+      tc_fence_after();
+      const int kv0 = k0 + tile(w, i) * kKv;
+      if (any) {  // a warp of padding rows only signals
+        float v[8][16];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) tmem_ld_32x32b_x16(tS + 16 * c, v[c]);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 8; ++c) pin(v[c]);
+        float mx = kNegBig;
+        if (__all_sync(0xffffffffu, kv0 + kKv - 1 <= limit)) {
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              v[c][e] *= a.scale_log2;
+              mx = fmaxf(mx, v[c][e]);
+            }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              v[c][e] = kv0 + 16 * c + e <= limit ? v[c][e] * a.scale_log2 : -INFINITY;
+              mx = fmaxf(mx, v[c][e]);
+            }
+        }
+        const float m_new = fmaxf(m, mx);
+        const bool grow = m_new > m + kLazy || i == 0;
+        const float alpha = grow ? exp2f(m - m_new) : 1.f;
+        if (i > 0 && __any_sync(0xffffffffu, grow)) {
+#pragma unroll 1
+          for (int c = 0; c < D; c += 16) {
+            float o[16];
+            tmem_ld_32x32b_x16(tO + c, o);
+            tmem_wait_ld();
+            pin(o);
+            uint32_t u[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(o[e] * alpha);
+            tmem_st_x16(tO + c, u);
+          }
+        }
+        if (grow) {
+          l *= alpha;
+          m = m_new;
+        }
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {  // 32 keys -> 16 columns of P
+          uint32_t u[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float p0 = exp2f(v[2 * c + (e >> 3)][(2 * e) & 15] - m);
+            const float p1 = exp2f(v[2 * c + (e >> 3)][(2 * e + 1) & 15] - m);
+            sum[e & 3] += p0 + p1;
+            u[e] = pack_bf16x2(p0, p1);  // rounded by 2^-8 at most; l keeps the fp32 sum
+          }
+          tmem_st_x16(tS + 16 * c, u);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_wait_st();
+      }
+      if (kv0 + kKv > k1) {  // V rows behind the last key: whatever they hold must not meet p = 0
+        const int tl = tile(w, i), s = tl % kStages;
+        if (!mbar_wait(&fullV[s], (tl / kStages) & 1, abort_flag, a.status, kStatusAttnTimeout)) failed = true;
+        for (int c = t; c < (kv0 + kKv - k1) * 8; c += kRows)
+#pragma unroll
+          for (int rg = 0; rg < D / 64; ++rg)
+            reinterpret_cast<uint4*>(sV + s * C::kTile + rg * C::kRegion + (k1 - kv0) * 128)[c] = make_uint4(0, 0, 0, 0);
+        fence_proxy_async();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_ready[w]);
+    }
+    if (!failed && n > 0 && !mbar_wait(&o_done[w], (n - 1) & 1, abort_flag, a.status, kStatusAttnTimeout)) failed = true;
+    failed = __any_sync(0xffffffffu, failed);
+    if (!failed && any) {
+      tc_fence_after();
+      const long part = kPair ? it.z : 2 * it.z + w;
+      const long at = (part * a.B * a.ql + token) * a.nq + h;
+      if (valid) a.part_ml[at] = make_float2(m, l);
+#pragma unroll 1
+      for (int c = 0; c < D; c += 16) {
+        float o[16];
+        if (n > 0) {
+          tmem_ld_32x32b_x16(tO + c, o);
+          tmem_wait_ld();
+          pin(o);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[e] = 0.f;
+        }
+        if (valid)
+#pragma unroll
+          for (int e = 0; e < 16; e += 4)
+            *reinterpret_cast<float4*>(a.part_o + at * D + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+}  // namespace tc
+
 // Each sequence's own keys, then the sum with the prefix.  grid (B, KV heads x row chunks, page splits), the splits of
 // a row one cluster.
 template <int D, int MT>
@@ -381,7 +777,7 @@ __global__ void __launch_bounds__(kWarps * 32)
   cg::cluster_group cl = cg::this_cluster();
   if (splits > 1) cl.sync();
   griddep_wait();
-  const int n_prefix = gr.prefix > 0 ? (gr.prefix + gr.chunk - 1) / gr.chunk : 0;
+  const int n_prefix = gr.prefix > 0 ? (gr.prefix + gr.chunk - 1) / gr.chunk * a.parts : 0;
   // one warp per row: the weights of all parts, then the sum; the rows are dealt over the CTAs of the cluster
   for (int r = me * kWarps + warp_id(); r < rows; r += splits * kWarps) {
     const int lane = lane_id();
@@ -435,6 +831,15 @@ void launch_prefix(const CUtensorMap& tm, const Args& a, int items, cudaStream_t
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
+template <int D, bool kPair>
+void launch_prefix_tc(const CUtensorMap& tm, const Args& a, int items, cudaStream_t stream) {
+  constexpr int smem = tc::Cfg<D>::kSmem;
+  C10_CUDA_CHECK(
+      cudaFuncSetAttribute(tc::prefix_tc_kernel<D, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  tc::prefix_tc_kernel<D, kPair><<<dim3(items, a.nkv), tc::kThreads, smem, stream>>>(tm, a);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
 template <int D, int MT>
 void launch_suffix(const CUtensorMap& tm, const Args& a, int splits, bool dependent, cudaStream_t stream) {
   constexpr int smem = stream_smem<D, MT>();
@@ -465,7 +870,9 @@ template <int D>
 void run(const CUtensorMap& tm, const Args& a, int items, int tile_rows, int suffix_splits, cudaStream_t stream) {
   if (items > 0) {
     if (tile_rows == 16) launch_prefix<D, 1>(tm, a, items, stream);
-    else launch_prefix<D, 2>(tm, a, items, stream);
+    else if (tile_rows == 32) launch_prefix<D, 2>(tm, a, items, stream);
+    else if (tile_rows == 128) launch_prefix_tc<D, false>(tm, a, items, stream);
+    else launch_prefix_tc<D, true>(tm, a, items, stream);
   }
   if (a.ql * (a.nq / a.nkv) <= 16) launch_suffix<D, 1>(tm, a, suffix_splits, items > 0, stream);
   else launch_suffix<D, 2>(tm, a, suffix_splits, items > 0, stream);
@@ -508,7 +915,7 @@ void shared_prefix_attention(const torch::Tensor& q, const torch::Tensor& kv_cac
                   groups.scalar_type() == at::kInt && groups.dim() == 2 && groups.size(1) == 4 &&
                   groups.is_contiguous(),
               "items and groups must be a plan's");
-  SP_CHECK(tile_rows == 16 || tile_rows == 32, "unknown row tile");
+  SP_CHECK(tile_rows == 16 || tile_rows == 32 || tile_rows == 128 || tile_rows == 256, "unknown row tile");
   SP_CHECK(suffix_splits == 1 || suffix_splits == 2 || suffix_splits == 4 || suffix_splits == 8, "suffix_splits must be 1, 2, 4 or 8");
   const uint64_t rows = (uint64_t)kv_cache.size(1) * 2 * nkv * PAGE;
   SP_CHECK(rows < (1ull << 31), "kv_cache has too many rows per layer for 32-bit tile coordinates");
@@ -540,6 +947,8 @@ void shared_prefix_attention(const torch::Tensor& q, const torch::Tensor& kv_cac
   a.NB = int(kv_cache.size(1));
   a.scale_log2 = float(scale * 1.4426950408889634);
   a.status = status_word(q.get_device());
+  a.parts = tile_rows == 128 ? 2 : 1;
+  prefix_splits *= a.parts;
   // partial sums of the prefix: every (split, row) that the suffix kernel reads is written by an item
   auto ws = torch::empty({prefix_splits * T * nq * (D + 2)}, q.options().dtype(at::kFloat));
   a.part_o = ws.data_ptr<float>();
