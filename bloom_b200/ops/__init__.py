@@ -596,7 +596,7 @@ def shared_prefix_plan(group_sizes, prefix_lens, *, num_q_heads: int, num_kv_hea
     # Rows of a CTA's tile.  Up to 32 stream past the keys on mma.sync (several CTAs per SM); more go to tcgen05,
     # in one 128-row tile or in pairs of them.
     most = max(rows, default=0)
-    p.tile_rows = 16 if most <= 16 else 32 if most <= 32 else 128 if most <= 128 else 256
+    p.tile_rows = next((t for t in (8, 16, 32, 128) if most <= t), 256)
     tiles = [-(-r // p.tile_rows) for r in rows]
     step, slots = (64, 2 * sms) if p.tile_rows <= 32 else (128 if p.tile_rows == 256 else 256, sms)
     chunk = _prefix_chunk(prefix, [t * num_kv_heads for t in tiles], step, slots)

@@ -32,13 +32,17 @@ namespace shared_prefix {
 
 constexpr int PAGE = 16;
 constexpr float kNegBig = -1e30f;
-constexpr int kWarps = 4, kStages = 3;  // streaming kernels: warps and ring depth per warp
+constexpr int kWarps = 4;  // of a streaming CTA
+// CTAs per SM that the registers are kept low enough for: O alone takes NT * D / 4 of them
+template <int D, int NT>
+constexpr int kCtas = D * NT >= 512 ? 2 : D * NT >= 256 ? 3 : 4;
 
 struct Group {  // one row of plan.groups
   int first, members, prefix, chunk;  // first sequence, sequences, shared tokens, prefix tokens per split
 };
 
 struct Args {
+  const __nv_bfloat16* kv; // this layer's pages [NB, 2, nkv, 16, D]
   const __nv_bfloat16* q;  // [B * ql, nq, D]
   long q_stride;           // elements between token rows
   __nv_bfloat16* out;
@@ -58,16 +62,6 @@ struct Args {
   int* status;
 };
 
-__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
-               : "r"(addr));
-}
-__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
-               : "r"(addr));
-}
 __device__ __forceinline__ void mma_bf16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
@@ -76,12 +70,6 @@ __device__ __forceinline__ void mma_bf16_16816(float (&d)[4], const uint32_t (&a
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
-// Byte address of element (tok, d), d a multiple of 8, of a page that TMA wrote as 2 KB boxes of 64 dims with the
-// 128-byte swizzle.
-__device__ __forceinline__ uint32_t page_addr(uint32_t base, int tok, int d) {
-  return base + ((d >> 6) << 11) + (tok << 7) + (((((d & 63) >> 3) ^ (tok & 7))) << 4);
-}
 
 // Length of sequence b, kept inside its table row.
 __device__ __forceinline__ int seq_len(const Args& a, int b) {
@@ -118,185 +106,202 @@ __device__ __forceinline__ int2 prefix_holder(const Args& a, const Group& g) {
   return make_int2(g.first + int(0xffffffffu - unsigned(best)), int(best >> 32));
 }
 
+// Shared memory of a streaming CTA: the query rows (where they do not stay in registers), and one partial result per
+// warp and row.
 template <int D>
-constexpr int stage_bytes() { return 2 * PAGE * D * 2; }
-template <int D, int MT>
-constexpr int stream_smem() {
-  constexpr int ring = kWarps * kStages * stage_bytes<D>(), merge = kWarps * MT * 16 * (D + 2) * 4;
-  return (ring > merge ? ring : merge) + kWarps * kStages * 8 + 1024;
-}
+constexpr int kQStride = D * 2 + 64;  // bytes of a query row: neighbouring rows start in different banks
+template <int D, int NT>
+constexpr int q_bytes() { return NT > 1 ? NT * 8 * kQStride<D> : 0; }
+template <int D, int NT>
+constexpr int stream_smem(int rows) { return q_bytes<D, NT>() + kWarps * rows * (D + 2) * 4; }
 
-// Streams keys [k_begin, k_end) of one KV head past up to MT * 16 packed query rows (row r: token q0 + r / G, q head
-// kh * G + r % G; limit(r): the last key that it sees) and leaves, in shared memory, row r's O[D], m, l at
-// merged + r * (D + 2).  Each warp streams every kWarps-th page through its own TMA ring; the rows are the M dimension
-// of m16n8k16 MMAs, so a page is read once for all of them.
-template <int D, int MT, typename Limit>
-__device__ float* stream(const CUtensorMap& tm, const Args& a, uint8_t* smem, int* abort_flag, const int* row, int kh,
-                         long q0, int r0, int rows, int k_begin, int k_end, Limit&& limit_of) {
-  constexpr int kStage = stage_bytes<D>(), kPageB = PAGE * D * 2, RS = D + 2;
-  constexpr int ring = kWarps * kStages * kStage, merge = kWarps * MT * 16 * RS * 4;
+// Streams keys [k_begin, k_end) of one KV head past up to NT * 8 packed query rows (row r: token q0 + (r0 + r) / G,
+// q head kh * G + (r0 + r) % G; limit(r): the last key that it sees) and leaves, in shared memory, row r's O[D], m, l at
+// result + r * (D + 2).  A page is read once for all rows.
+//
+// The products are formed transposed, S^T = K Q^T and O^T = V^T P^T, so that keys and dims fill the 16-row side of
+// m16n8k16 and 4 to 8 query rows (a GQA group) fill its 8-column side: half the MMAs and half the registers for O of
+// the other way round.  Each warp takes every kWarps-th page and loads it straight into A fragments, 16 bytes a load:
+// the dims of Q K^T may be summed in any order, so a thread's 8 contiguous dims of a key are fragments of two MMAs (Q in
+// the same order); for P V the 8 contiguous dims of 4 keys are interleaved by byte permutes.  P^T moves from
+// accumulator to B fragments by an 8x8 transpose of the warp.  The next page's K is requested once S is formed, its V
+// once P V is issued: 8 KB in flight per warp without shared memory, barriers or ldmatrix.
+template <int D, int NT, typename Limit>
+__device__ float* stream(const Args& a, uint8_t* smem, const int* row, int kh, long q0, int r0, int rows, int k_begin,
+                         int k_end, Limit&& limit_of) {
+  constexpr int RS = D + 2, NC = D / 32, NB = D / 64;
   const int warp = warp_id(), lane = lane_id(), g = lane >> 2, t4 = lane & 3;
   const int G = a.nq / a.nkv;
-  uint8_t* wsm = smem + warp * kStages * kStage;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (ring > merge ? ring : merge)) + warp * kStages;
   const int p0 = k_begin / PAGE, p1 = k_end > k_begin ? (k_end + PAGE - 1) / PAGE : p0;
   const int first = p0 + warp;
-  const int my_n = p1 > first ? (p1 - first + kWarps - 1) / kWarps : 0;
-  if (lane == 0) {
-    for (int s = 0; s < kStages; ++s) mbar_init(&bars[s], 1);
-    fence_barrier_init();
-  }
-  __syncthreads();
-  auto issue = [&](int i) {
-    const int s = i % kStages;
-    const int blk = block_id(a, row, first + i * kWarps);
-    const int rowK = (blk * 2 * a.nkv + kh) * PAGE, rowV = ((blk * 2 + 1) * a.nkv + kh) * PAGE;
-    uint8_t* st = wsm + s * kStage;
-    mbar_arrive_expect_tx(&bars[s], kStage);
-    tma_load_2d(st, &tm, &bars[s], 0, rowK);
-    if constexpr (D == 128) tma_load_2d(st + 2048, &tm, &bars[s], 64, rowK);
-    tma_load_2d(st + kPageB, &tm, &bars[s], 0, rowV);
-    if constexpr (D == 128) tma_load_2d(st + kPageB + 2048, &tm, &bars[s], 64, rowV);
-  };
-  if (lane == 0)
-    for (int i = 0; i < kStages && i < my_n; ++i) issue(i);
+  const int n = p1 > first ? (p1 - first + kWarps - 1) / kWarps : 0;
 
-  uint32_t qf[MT][D / 16][4];
-  int limit[MT][2];
+  int ids = 0;  // block ids of this warp's next 32 pages, one per lane
+  auto fetch_ids = [&](int i) {
+    const int p = first + (i + lane) * kWarps;
+    ids = p < p1 ? block_id(a, row, p) : 0;
+  };
+  auto page_of = [&](int i, int kv) {
+    const long blk = __shfl_sync(0xffffffffu, ids, i & 31);
+    return a.kv + ((blk * 2 + kv) * a.nkv + kh) * (PAGE * D);
+  };
+  uint4 kf[2][NC], vf[4][NB];
+  auto load_k = [&](int i) {  // keys g and g + 8
+    const __nv_bfloat16* p = page_of(i, 0) + g * D + t4 * 8;
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int hr = 0; hr < 2; ++hr) {
-      const int r = mt * 16 + g + 8 * hr;
-      const __nv_bfloat16* qrow = nullptr;
-      limit[mt][hr] = -1;
-      if (r < rows) {
-        qrow = a.q + (q0 + (r0 + r) / G) * a.q_stride + (kh * G + (r0 + r) % G) * D;
-        limit[mt][hr] = min(limit_of(r), k_end - 1);
-      }
+      for (int c = 0; c < NC; ++c) kf[h][c] = __ldg(reinterpret_cast<const uint4*>(p + h * 8 * D + c * 32));
+  };
+  auto load_v = [&](int i) {  // keys 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9 of the page
+    const __nv_bfloat16* p = page_of(i, 1) + 2 * t4 * D + g * 8;
+    const int left = k_end - (first + i * kWarps) * PAGE;  // slots at or behind the last key may hold anything: zeros
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        const int d = ks * 16 + 2 * t4;
-        qf[mt][ks][hr] = qrow ? *reinterpret_cast<const uint32_t*>(qrow + d) : 0u;
-        qf[mt][ks][hr + 2] = qrow ? *reinterpret_cast<const uint32_t*>(qrow + d + 8) : 0u;
-      }
+    for (int k = 0; k < 4; ++k) {
+      const int tok = (k & 1) + 8 * (k >> 1);
+#pragma unroll
+      for (int d = 0; d < NB; ++d)
+        vf[k][d] = 2 * t4 + tok < left ? __ldg(reinterpret_cast<const uint4*>(p + tok * D + d * 64))
+                                       : make_uint4(0, 0, 0, 0);
     }
-  float m_run[MT][2], l_run[MT][2], o[MT][D / 8][4];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    m_run[mt][0] = m_run[mt][1] = kNegBig;
-    l_run[mt][0] = l_run[mt][1] = 0.f;
-#pragma unroll
-    for (int n = 0; n < D / 8; ++n) o[mt][n][0] = o[mt][n][1] = o[mt][n][2] = o[mt][n][3] = 0.f;
+  };
+  if (n > 0) {
+    fetch_ids(0);
+    load_k(0);
+    load_v(0);
   }
-  int i = 0;
-  for (; i < my_n; ++i) {
-    const int s = i % kStages;
-    if (!mbar_wait(&bars[s], (i / kStages) & 1, abort_flag, a.status, kStatusAttnTimeout)) break;
-    const uint32_t sK = smem_u32(wsm + s * kStage), sV = sK + kPageB;
+  // Q^T fragments: row g of each 8-row tile, this thread's 8 dims of each 32
+  auto q_row = [&](int r) { return a.q + (q0 + (r0 + r) / G) * a.q_stride + (kh * G + (r0 + r) % G) * D; };
+  uint4 qr[NC];
+  if constexpr (NT == 1) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      qr[c] = g < rows ? __ldg(reinterpret_cast<const uint4*>(q_row(g) + c * 32 + t4 * 8)) : make_uint4(0, 0, 0, 0);
+  } else {
+    for (int c = threadIdx.x; c < NT * 8 * (D / 8); c += kWarps * 32) {
+      const int r = c / (D / 8), d = c % (D / 8);
+      *reinterpret_cast<uint4*>(smem + r * kQStride<D> + d * 16) =
+          r < rows ? __ldg(reinterpret_cast<const uint4*>(q_row(r) + d * 8)) : make_uint4(0, 0, 0, 0);
+    }
+    __syncthreads();
+  }
+  int limit[NT][2], low = 0x7fffffff;  // of rows 8 nt + 2 t4 + e
+  float m_run[NT][2], l_run[NT][2], o[NT][D / 16][4];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = nt * 8 + 2 * t4 + e;
+      limit[nt][e] = r < rows ? min(limit_of(r), k_end - 1) : 0x7fffffff;  // padding rows are not masked, nor used
+      low = min(low, limit[nt][e]);
+      m_run[nt][e] = kNegBig;
+      l_run[nt][e] = 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
+  }
+  low = __reduce_min_sync(0xffffffffu, low);
+  for (int i = 0; i < n; ++i) {
     const int tok0 = (first + i * kWarps) * PAGE;
-    if (tok0 + PAGE > k_end) {  // V rows behind the last key: whatever they hold must not meet p = 0
-      for (int c = lane; c < PAGE * D / 8; c += 32) {
-        const int tok = c & 15, d = (c >> 4) * 8;
-        if (tok0 + tok >= k_end)
-          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(page_addr(sV, tok, d)), "r"(0) : "memory");
+    float sc[NT][4];  // [key g: rows 2 t4, 2 t4 + 1 | key g + 8: the same]
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const uint32_t a0[4] = {kf[0][c].x, kf[1][c].x, kf[0][c].y, kf[1][c].y};
+      const uint32_t a1[4] = {kf[0][c].z, kf[1][c].z, kf[0][c].w, kf[1][c].w};
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        uint4 q;
+        if constexpr (NT == 1) q = qr[c];
+        else q = *reinterpret_cast<const uint4*>(smem + (nt * 8 + g) * kQStride<D> + c * 64 + t4 * 16);
+        mma_bf16_16816(sc[nt], a0, q.x, q.y);
+        mma_bf16_16816(sc[nt], a1, q.z, q.w);
       }
-      __syncwarp();
     }
-    float sc[MT][2][4];
+    if (i + 1 < n) {
+      if (((i + 1) & 31) == 0) fetch_ids(i + 1);
+      load_k(i + 1);
+    }
+    const bool whole = tok0 >= k_begin && tok0 + PAGE - 1 <= low;  // every row sees every key of the page
+    uint32_t pb[NT][2];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int nt = 0; nt < NT; ++nt) {
+      float mx[2];
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt) sc[mt][nt][0] = sc[mt][nt][1] = sc[mt][nt][2] = sc[mt][nt][3] = 0.f;
+      for (int e = 0; e < 2; ++e) {
 #pragma unroll
-    for (int j = 0; j < D / 32; ++j)
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
-        uint32_t b0, b1, b2, b3;
-        ldsm_x4(page_addr(sK, 8 * nt + (lane & 7), 32 * j + 8 * (lane >> 3)), b0, b1, b2, b3);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          mma_bf16_16816(sc[mt][nt], qf[mt][2 * j], b0, b1);
-          mma_bf16_16816(sc[mt][nt], qf[mt][2 * j + 1], b2, b3);
+        for (int h = 0; h < 2; ++h) {
+          const int idx = tok0 + g + 8 * h;
+          float& x = sc[nt][2 * h + e];
+          x *= a.scale_log2;
+          if (!whole && (idx < k_begin || idx > limit[nt][e])) x = -INFINITY;
         }
+        mx[e] = fmaxf(sc[nt][e], sc[nt][2 + e]);
       }
-    uint32_t pa[MT][4];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+      for (int w = 4; w < 32; w <<= 1) {
+        mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], w));
+        mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], w));
+      }
+      const bool grows = mx[0] > m_run[nt][0] || mx[1] > m_run[nt][1];
+      if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
-      for (int hr = 0; hr < 2; ++hr) {
-        float x[4], mx = kNegBig;
+        for (int e = 0; e < 2; ++e) {
+          const float m_new = fmaxf(m_run[nt][e], mx[e]);
+          const float alpha = exp2f(m_run[nt][e] - m_new);
+          m_run[nt][e] = m_new;
+          l_run[nt][e] *= alpha;
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int idx = tok0 + 8 * nt + 2 * t4 + e;
-            const bool sees = idx >= k_begin && idx <= limit[mt][hr];
-            const float v = sees ? sc[mt][nt][2 * hr + e] * a.scale_log2 : -INFINITY;
-            x[nt * 2 + e] = v;
-            mx = fmaxf(mx, v);
+          for (int j = 0; j < D / 16; ++j) {
+            o[nt][j][e] *= alpha;
+            o[nt][j][2 + e] *= alpha;
           }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float m_new = fmaxf(m_run[mt][hr], mx);
-        const float alpha = exp2f(m_run[mt][hr] - m_new);
-        m_run[mt][hr] = m_new;
-        float ps = 0.f;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          x[k] = exp2f(x[k] - m_new);
-          ps += x[k];
         }
-        l_run[mt][hr] = l_run[mt][hr] * alpha + ps;
+      }
 #pragma unroll
-        for (int n = 0; n < D / 8; ++n) {
-          o[mt][n][2 * hr] *= alpha;
-          o[mt][n][2 * hr + 1] *= alpha;
-        }
+      for (int h = 0; h < 2; ++h) {
+        const float x0 = exp2f(sc[nt][2 * h] - m_run[nt][0]), x1 = exp2f(sc[nt][2 * h + 1] - m_run[nt][1]);
+        l_run[nt][0] += x0;
+        l_run[nt][1] += x1;
         // P is rounded to bf16 (2^-8 relative at most) for the tensor cores; l keeps the fp32 sum
-        pa[mt][hr] = pack_bf16x2(x[0], x[1]);
-        pa[mt][hr + 2] = pack_bf16x2(x[2], x[3]);
-      }
-#pragma unroll
-    for (int j = 0; j < D / 16; ++j) {
-      uint32_t b0, b1, b2, b3;
-      ldsm_x4_t(page_addr(sV, (lane & 7) + 8 * ((lane >> 3) & 1), 16 * j + 8 * (lane >> 4)), b0, b1, b2, b3);
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        mma_bf16_16816(o[mt][2 * j], pa[mt], b0, b1);
-        mma_bf16_16816(o[mt][2 * j + 1], pa[mt], b2, b3);
+        const uint32_t p = pack_bf16x2(x0, x1);
+        asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pb[nt][h]) : "r"(p));
       }
     }
-    __syncwarp();
-    if (lane == 0 && i + kStages < my_n) {
-      fence_proxy_async();
-      issue(i + kStages);
-    }
+#pragma unroll
+    for (int d = 0; d < NB; ++d)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {  // rows g and g + 8 of tile j are dims 64 d + 8 g + 2 j and the next
+        auto word = [&](const uint4& v) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; };
+        const uint32_t w0 = word(vf[0][d]), w1 = word(vf[1][d]), w2 = word(vf[2][d]), w3 = word(vf[3][d]);
+        const uint32_t av[4] = {__byte_perm(w0, w1, 0x5410), __byte_perm(w0, w1, 0x7632), __byte_perm(w2, w3, 0x5410),
+                                __byte_perm(w2, w3, 0x7632)};
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma_bf16_16816(o[nt][4 * d + j], av, pb[nt][0], pb[nt][1]);
+      }
+    if (i + 1 < n) load_v(i + 1);
   }
-  if (i < my_n && lane == 0)  // gave up: the loads in flight must land before the shared memory is reused
-    for (int k = i; k < my_n && k < i + kStages; ++k) mbar_drain(&bars[k % kStages], (k / kStages) & 1);
+  // the warps' results into shared memory, then summed into warp 0's place
+  float* cm = reinterpret_cast<float*>(smem + q_bytes<D, NT>());
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+  for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int hr = 0; hr < 2; ++hr) {
-      float l = l_run[mt][hr];
-      l += __shfl_xor_sync(0xffffffffu, l, 1);
-      l += __shfl_xor_sync(0xffffffffu, l, 2);
-      l_run[mt][hr] = l;
-    }
-  __syncthreads();
-  // the warps' results into the shared memory of the rings, then summed into warp 0's place
-  float* cm = reinterpret_cast<float*>(smem);
-  float* wbuf = cm + warp * (MT * 16 * RS);
+    for (int e = 0; e < 2; ++e) {
+      float l = l_run[nt][e];
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+      for (int w = 4; w < 32; w <<= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+      const int r = nt * 8 + 2 * t4 + e;
+      if (r < rows) {
+        float* w = cm + (warp * rows + r) * RS;
 #pragma unroll
-    for (int hr = 0; hr < 2; ++hr) {
-      const int r = mt * 16 + g + 8 * hr;
+        for (int d = 0; d < NB; ++d)
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n)
-        *reinterpret_cast<float2*>(wbuf + r * RS + 8 * n + 2 * t4) = make_float2(o[mt][n][2 * hr], o[mt][n][2 * hr + 1]);
-      if (t4 == 0) *reinterpret_cast<float2*>(wbuf + r * RS + D) = make_float2(m_run[mt][hr], l_run[mt][hr]);
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<float2*>(w + 64 * d + 8 * g + 2 * j) =
+                make_float2(o[nt][4 * d + j][e], o[nt][4 * d + j][2 + e]);
+        if (g == 0) *reinterpret_cast<float2*>(w + D) = make_float2(m_run[nt][e], l);
+      }
     }
   __syncthreads();
   // one warp per row: every lane reads the row's (m, l) of all warps before any lane writes the sums back
@@ -304,21 +309,20 @@ __device__ float* stream(const CUtensorMap& tm, const Args& a, uint8_t* smem, in
     float m[kWarps], M = kNegBig, L = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float2 ml = *reinterpret_cast<const float2*>(cm + (w * MT * 16 + r) * RS + D);
-      m[w] = ml.x;
-      M = fmaxf(M, ml.x);
+      m[w] = cm[(w * rows + r) * RS + D];
+      M = fmaxf(M, m[w]);
     }
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       m[w] = exp2f(m[w] - M);
-      L += cm[(w * MT * 16 + r) * RS + D + 1] * m[w];
+      L += cm[(w * rows + r) * RS + D + 1] * m[w];
     }
     __syncwarp();
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
       float O = 0.f;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) O += cm[(w * MT * 16 + r) * RS + c * 32 + lane] * m[w];
+      for (int w = 0; w < kWarps; ++w) O += cm[(w * rows + r) * RS + c * 32 + lane] * m[w];
       cm[r * RS + c * 32 + lane] = O;
     }
     if (lane == 0) *reinterpret_cast<float2*>(cm + r * RS + D) = make_float2(M, L);
@@ -327,24 +331,19 @@ __device__ float* stream(const CUtensorMap& tm, const Args& a, uint8_t* smem, in
   return cm;
 }
 
-// Prefix work of groups with few rows: the keys stream past at most MT * 16 of them.  grid (items, KV heads).
-template <int D, int MT>
-__global__ void __launch_bounds__(kWarps * 32)
-    prefix_stream_kernel(const __grid_constant__ CUtensorMap tm, const Args a) {
+// Prefix work of groups with few rows: the keys stream past at most NT * 8 of them.  grid (items, KV heads).
+template <int D, int NT>
+__global__ void __launch_bounds__(kWarps * 32, kCtas<D, NT>) prefix_stream_kernel(const Args a) {
   griddep_launch_dependents();
-  extern __shared__ uint8_t raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  __shared__ int abort_flag;
-  if (threadIdx.x == 0) abort_flag = 0;
+  extern __shared__ __align__(16) uint8_t smem[];
   const int4 it = a.items[blockIdx.x];
   const Group gr = a.groups[it.x];
   const int kh = blockIdx.y, G = a.nq / a.nkv;
   const int2 hold = prefix_holder(a, gr);
   const int k0 = min(it.z * gr.chunk, hold.y), k1 = min(k0 + gr.chunk, hold.y);
-  const int rows = min(MT * 16, gr.members * a.ql * G - it.y);
+  const int rows = min(NT * 8, gr.members * a.ql * G - it.y);
   const long q0 = (long)gr.first * a.ql;
-  const float* res = stream<D, MT>(tm, a, smem, &abort_flag, a.table + hold.x * a.table_stride, kh, q0, it.y, rows, k0,
-                                   k1, [&](int r) {
+  const float* res = stream<D, NT>(a, smem, a.table + hold.x * a.table_stride, kh, q0, it.y, rows, k0, k1, [&](int r) {
                                      const int tok = (it.y + r) / G;
                                      return seq_len(a, gr.first + tok / a.ql) - a.ql + tok % a.ql;
                                    });
@@ -360,30 +359,31 @@ __global__ void __launch_bounds__(kWarps * 32)
 
 // ---------------------------------------------------------------- prefix on tcgen05
 // Groups with more rows than a streaming CTA holds: S = Q K^T and O += P V on the 5th-generation tensor cores, with
-// 128 rows per softmax warpgroup, one thread per row (no exchange between threads).  A CTA runs two such streams that
-// take turns on the tensor pipe, one stream's softmax under the other's MMAs:
+// 128 rows per softmax warpgroup, one thread per row (no exchange between threads).  A CTA runs two such streams:
 //   pair   (256-row items)  two row tiles over the same K / V tiles, so each K / V tile serves 256 rows
 //   single (128-row items)  one row tile, the streams take alternate K / V tiles and leave one partial sum each
-// TMEM: S0, S1, O0, O1 of 128 columns; P (bf16, two keys per column) is written over the first half of its S and
-// read from there as the A operand, so it never goes through shared memory.  S(i + 1) of a stream is issued only after
-// its P V(i) has completed, which also makes O safe to rescale when S(i + 1) is seen.  The running max is lazy: O is
-// rescaled only when a row's max grows by more than 2^8.
+// Tiles of 64 keys, so that TMEM holds two S buffers per stream beside the two O (4 x 64 + 2 x 128 columns): S(i + 1)
+// is formed while the softmax works on S(i), and the softmax never waits for a product.  P (bf16, two keys per column)
+// is written over the first half of its S and read from there as the A operand.  With 128-key tiles and one S buffer
+// per stream, S(i + 1) had to wait for P V(i), and each tile's softmax for both: 6,300 cycles per 128 keys of a pair,
+// half of them waiting.  The running max is lazy: O is rescaled (and P V(i - 1) waited for) only when a row's max
+// grows by more than 2^8.
 // Warps 0-7 softmax and epilogue, warp 8 TMA producer and TMEM owner, warp 9 issues the MMAs of both streams from an
 // event loop over their barriers.
 namespace tc {
 
-constexpr int kRows = 128, kKv = 128;
+constexpr int kRows = 128, kKv = 64;
 constexpr int kThreads = 256 + 64;
 constexpr int kTmemCols = 512;
 constexpr float kLazy = 8.f;  // log2 units
 
 template <int D>
 struct Cfg {
-  static constexpr int kRegion = kKv * 128;       // 64 dims of a K or V tile: 128 token rows of 128 bytes
+  static constexpr int kRegion = kKv * 128;       // 64 dims of a K or V tile: token rows of 128 bytes
   static constexpr int kTile = kKv * D * 2;
   static constexpr int kQ = kRows * D * 2;
-  static constexpr int kStages = D == 128 ? 2 : 4;  // of the K ring and of the V ring
-  static constexpr int kSmem = 2 * kQ + 2 * kStages * kTile + 256 + 1024;
+  static constexpr int kStages = D == 128 ? 4 : 8;  // of the K ring and of the V ring
+  static constexpr int kSmem = 2 * kQ + 2 * kStages * kTile + 512 + 1024;
 };
 
 __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
@@ -440,9 +440,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* sK = smem + 2 * C::kQ;
   uint8_t* sV = sK + kStages * C::kTile;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sV + kStages * C::kTile);
-  uint64_t *fullK = bars, *emptyK = bars + 4, *fullV = bars + 8, *emptyV = bars + 12;
-  uint64_t *s_done = bars + 16, *p_ready = bars + 18, *o_done = bars + 20, *q_ready = bars + 22, *drain = bars + 23;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
+  uint64_t *fullK = bars, *emptyK = bars + 8, *fullV = bars + 16, *emptyV = bars + 24;
+  // [2 * stream + (tile & 1)]
+  uint64_t *s_done = bars + 32, *p_ready = bars + 36, *o_done = bars + 40;
+  uint64_t *q_ready = bars + 44, *drain = bars + 45;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 46);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = warp_id(), lane = lane_id();
@@ -466,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&emptyK[s], two ? 2 : 1);
       mbar_init(&emptyV[s], two ? 2 : 1);
     }
-    for (int w = 0; w < 2; ++w) {
+    for (int w = 0; w < 4; ++w) {
       mbar_init(&s_done[w], 1);
       mbar_init(&p_ready[w], 4);
       mbar_init(&o_done[w], 1);
@@ -483,130 +485,139 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;  // S_w at 128 w, O_w at 256 + 128 w
+  const uint32_t tmem = *tmem_slot;  // S(i) of stream w at 128 w + 64 (i & 1), O at 256 + 128 w
 
   if (warp == 8) {
-    if (lane == 0) {
-      const int n_pages = (k1 + PAGE - 1) / PAGE;
-      auto load = [&](int t, uint8_t* dst, uint64_t* bar, int kv) {
-        int ids[kKv / PAGE];
-#pragma unroll
-        for (int p = 0; p < kKv / PAGE; ++p) {
-          const int page = k0 / PAGE + t * (kKv / PAGE) + p;
-          ids[p] = block_id(a, table, page < n_pages ? page : k0 / PAGE);  // behind the end: any page, it is masked
-        }
-        mbar_arrive_expect_tx(bar, C::kTile);
-#pragma unroll
-        for (int p = 0; p < kKv / PAGE; ++p) {
-          const int row = ((ids[p] * 2 + kv) * a.nkv + kh) * PAGE;
-#pragma unroll
-          for (int r = 0; r < D / 64; ++r) tma_load_2d(dst + r * C::kRegion + p * 2048, &tm, bar, 64 * r, row);
-        }
-      };
-      int nK = 0, nV = 0;
-      bool ok = true;
-      uint64_t t_prog = globaltimer_ns();
-      uint32_t spins = 0;
-      while (ok && (nK < n_kt || nV < n_kt)) {  // the rings advance on their own; V never runs ahead of K
-        bool progressed = false;
-        if (nK < n_kt && mbar_test(&emptyK[nK % kStages], ((nK / kStages) & 1) ^ 1u)) {
-          load(nK, sK + nK % kStages * C::kTile, &fullK[nK % kStages], 0);
-          ++nK;
-          progressed = true;
-        }
-        if (nV < nK && mbar_test(&emptyV[nV % kStages], ((nV / kStages) & 1) ^ 1u)) {
-          load(nV, sV + nV % kStages * C::kTile, &fullV[nV % kStages], 1);
-          ++nV;
-          progressed = true;
-        }
-        if (progressed) {
-          t_prog = globaltimer_ns();
-        } else if ((++spins & 31u) == 0) {
-          if (*abort_flag) {
-            ok = false;
-          } else if (globaltimer_ns() - t_prog > kLocalWaitTimeoutNs) {
+    // Lane p * (D / 64) + r brings 64 dims of page p of a tile.
+    constexpr int kBoxes = kKv / PAGE * (D / 64);
+    const int n_pages = (k1 + PAGE - 1) / PAGE, rg = lane % (D / 64);
+    auto fetch_id = [&](int t) {  // behind the end: any page, it is masked
+      const int page = k0 / PAGE + t * (kKv / PAGE) + lane / (D / 64);
+      return lane < kBoxes && t < n_kt ? block_id(a, table, page < n_pages ? page : k0 / PAGE) : 0;
+    };
+    auto load = [&](int id, uint8_t* dst, uint64_t* bar, int kv) {
+      if (lane == 0) mbar_arrive_expect_tx(bar, C::kTile);
+      __syncwarp();
+      if (lane < kBoxes)
+        tma_load_2d(dst + rg * C::kRegion + lane / (D / 64) * 2048, &tm, bar, 64 * rg,
+                    ((id * 2 + kv) * a.nkv + kh) * PAGE);
+    };
+    auto free_slot = [&](uint64_t* bar, int n) {  // one answer for the warp
+      return __shfl_sync(0xffffffffu, int(mbar_test(&bar[n % kStages], ((n / kStages) & 1) ^ 1u)), 0) != 0;
+    };
+    int nK = 0, nV = 0, idK = fetch_id(0), idV = idK;
+    bool ok = true;
+    uint64_t t_stall = 0;
+    uint32_t spins = 0;  // since the last progress
+    while (ok && (nK < n_kt || nV < n_kt)) {  // the rings advance on their own; V never runs ahead of K
+      bool progressed = false;
+      if (nK < n_kt && free_slot(emptyK, nK)) {
+        load(idK, sK + nK % kStages * C::kTile, &fullK[nK % kStages], 0);
+        idK = fetch_id(++nK);
+        progressed = true;
+      }
+      if (nV < nK && free_slot(emptyV, nV)) {
+        load(idV, sV + nV % kStages * C::kTile, &fullV[nV % kStages], 1);
+        idV = fetch_id(++nV);
+        progressed = true;
+      }
+      if (progressed) {
+        spins = 0;
+      } else if ((++spins & 63u) == 0) {
+        bool stop = false;
+        if (lane == 0) {
+          stop = *abort_flag;
+          if (spins == 64) t_stall = globaltimer_ns();
+          if (!stop && globaltimer_ns() - t_stall > kLocalWaitTimeoutNs) {
             *abort_flag = 1;
             atomicOr(a.status, kStatusAttnTimeout);
-            ok = false;
+            stop = true;
           }
         }
-      }
-      if (!ok) {  // the loads in flight land before the block leaves (bounded)
-        for (int j = max(0, nK - kStages); j < nK; ++j) mbar_drain(&fullK[j % kStages], (j / kStages) & 1);
-        for (int j = max(0, nV - kStages); j < nV; ++j) mbar_drain(&fullV[j % kStages], (j / kStages) & 1);
+        ok = !__shfl_sync(0xffffffffu, int(stop), 0);
       }
     }
+    if (!ok && lane == 0) {  // the loads in flight land before the block leaves (bounded)
+      for (int j = max(0, nK - kStages); j < nK; ++j) mbar_drain(&fullK[j % kStages], (j / kStages) & 1);
+      for (int j = max(0, nV - kStages); j < nV; ++j) mbar_drain(&fullV[j % kStages], (j / kStages) & 1);
+    }
   } else if (warp == 9) {
-    if (lane == 0 && n_kt > 0) {
+    // The whole warp runs the loop and one elected lane issues: operands of tcgen05.mma live in uniform registers, and
+    // in a branch on the lane every one of them is moved there for every instruction (90 cycles an MMA for S, 300 for
+    // P V, so that issuing took three times as long as the tensor pipe's work).  Answers of barriers are broadcast,
+    // which keeps the loop's state uniform.
+    if (n_kt > 0) {
+      auto done = [&](uint64_t* bar, uint32_t parity) {
+        return __shfl_sync(0xffffffffu, int(mbar_test(bar, parity)), 0) != 0;
+      };
       constexpr uint32_t idS = umma_idesc_bf16(kRows, kKv);
       constexpr uint32_t idO = umma_idesc_bf16(kRows, D) | (1u << 16);  // B is MN-major
-      bool ok = mbar_wait(q_ready, 0, abort_flag, a.status, kStatusAttnTimeout), issued = false;
-      auto issue_s = [&](int w, int t) {
-        tc_fence_after();
-        const int s = t % kStages;
-        const uint32_t kb = smem_u32(sK + s * C::kTile), qb = smem_u32(sQ + (kPair ? w * C::kQ : 0));
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
-          umma_f16(tmem + 128 * w, umma_desc_sw128(qb + (kk >> 2) * (kRows * 128)) + 2 * (kk & 3),
-                   umma_desc_sw128(kb + (kk >> 2) * C::kRegion) + 2 * (kk & 3), idS, kk > 0 ? 1u : 0u);
-        umma_commit(&s_done[w]);
-        umma_commit(&emptyK[s]);
-        issued = true;
-      };
-      // per stream: the tile in work, and whether its P V has been issued
-      int i[2] = {0, 0};
-      bool pv[2] = {false, false};
-      int left = 0;
-      for (int w = 0; w < 2 && ok; ++w)
-        if (count(w) > 0) {
-          ++left;
-          const int t = tile(w, 0);
-          ok = mbar_wait(&fullK[t % kStages], (t / kStages) & 1, abort_flag, a.status, kStatusAttnTimeout);
-          if (ok) issue_s(w, t);
-        }
-      uint64_t t_prog = globaltimer_ns();
-      uint32_t spins = 0;
+      bool issued = false;
+      bool ok = __shfl_sync(0xffffffffu, int(mbar_wait(q_ready, 0, abort_flag, a.status, kStatusAttnTimeout)), 0) != 0;
+      // per stream: the next tile whose S, and whose P V, is to be issued
+      int iS[2] = {0, 0}, iP[2] = {0, 0};
+      int left = (count(0) > 0) + (count(1) > 0);
+      uint64_t t_stall = 0;
+      uint32_t spins = 0;  // since the last progress
       while (ok && left > 0) {
         bool progressed = false;
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-          if (i[w] >= count(w)) continue;
-          if (!pv[w]) {
-            const int t = tile(w, i[w]), s = t % kStages;
-            if (!mbar_test(&p_ready[w], i[w] & 1) || !mbar_test(&fullV[s], (t / kStages) & 1)) continue;
+          const int i = iS[w], t = tile(w, i), s = t % kStages;
+          // the S buffer is free once P V of the tile two back has read P from it
+          if (i < count(w) && done(&fullK[s], (t / kStages) & 1) &&
+              (i < 2 || done(&o_done[2 * w + (i & 1)], ((i >> 1) - 1) & 1))) {
             tc_fence_after();
-            const uint32_t vb = smem_u32(sV + s * C::kTile);
+            const uint32_t kb = smem_u32(sK + s * C::kTile), qb = smem_u32(sQ + (kPair ? w * C::kQ : 0));
+            const uint64_t dq = umma_desc_sw128(qb), dk = umma_desc_sw128(kb);
+            if (elect_one_sync()) {
 #pragma unroll
-            for (int kk = 0; kk < kKv / 16; ++kk)
-              umma_f16_ts(tmem + 256 + 128 * w, tmem + 128 * w + 8 * kk, desc_mn(vb + kk * 16 * 128, C::kRegion), idO,
-                          (i[w] > 0 || kk > 0) ? 1u : 0u);
-            umma_commit(&o_done[w]);
-            umma_commit(&emptyV[s]);
-            pv[w] = true;
-            if (i[w] + 1 == count(w)) ++i[w], --left;  // the last one: the softmax warps wait for it
-          } else {
-            const int t = tile(w, i[w] + 1);
-            if (!mbar_test(&o_done[w], i[w] & 1) || !mbar_test(&fullK[t % kStages], (t / kStages) & 1)) continue;
-            issue_s(w, t);
-            ++i[w];
-            pv[w] = false;
+              for (int kk = 0; kk < D / 16; ++kk)  // descriptors count addresses in 16 bytes
+                umma_f16(tmem + 128 * w + 64 * (i & 1), dq + (kk >> 2) * (kRows * 8) + 2 * (kk & 3),
+                         dk + (kk >> 2) * (C::kRegion / 16) + 2 * (kk & 3), idS, kk > 0 ? 1u : 0u);
+              umma_commit(&s_done[2 * w + (i & 1)]);
+              umma_commit(&emptyK[s]);
+            }
+            __syncwarp();
+            ++iS[w];
+            issued = progressed = true;
           }
-          progressed = true;
+          const int j = iP[w], tv = tile(w, j), sv = tv % kStages;
+          if (j < iS[w] && done(&p_ready[2 * w + (j & 1)], (j >> 1) & 1) && done(&fullV[sv], (tv / kStages) & 1)) {
+            tc_fence_after();
+            const uint64_t dv = desc_mn(smem_u32(sV + sv * C::kTile), C::kRegion);
+            if (elect_one_sync()) {
+#pragma unroll
+              for (int kk = 0; kk < kKv / 16; ++kk)
+                umma_f16_ts(tmem + 256 + 128 * w, tmem + 128 * w + 64 * (j & 1) + 8 * kk, dv + kk * (16 * 128 / 16), idO,
+                            (j > 0 || kk > 0) ? 1u : 0u);
+              umma_commit(&o_done[2 * w + (j & 1)]);
+              umma_commit(&emptyV[sv]);
+            }
+            __syncwarp();
+            if (++iP[w] == count(w)) --left;
+            progressed = true;
+          }
         }
         if (progressed) {
-          t_prog = globaltimer_ns();
-        } else if ((++spins & 31u) == 0) {
-          if (*abort_flag) {
-            ok = false;
-          } else if (globaltimer_ns() - t_prog > kLocalWaitTimeoutNs) {
-            *abort_flag = 1;
-            atomicOr(a.status, kStatusAttnTimeout);
-            ok = false;
+          spins = 0;
+        } else if ((++spins & 63u) == 0) {
+          bool stop = false;
+          if (lane == 0) {
+            stop = *abort_flag;
+            if (spins == 64) t_stall = globaltimer_ns();
+            if (!stop && globaltimer_ns() - t_stall > kLocalWaitTimeoutNs) {
+              *abort_flag = 1;
+              atomicOr(a.status, kStatusAttnTimeout);
+              stop = true;
+            }
           }
+          ok = !__shfl_sync(0xffffffffu, int(stop), 0);
         }
       }
       if (!ok && issued) {  // what was issued completes before TMEM is freed
-        umma_commit(drain);
+        if (elect_one_sync()) umma_commit(drain);
+        __syncwarp();
         mbar_drain(drain, 0);
       }
     }
@@ -618,13 +629,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int tok = (valid ? r : 0) / G;
     const long token = (long)gr.first * a.ql + tok;
     const int h = kh * G + (valid ? r : 0) % G;
+    // scores are scaled by |scale| inside the exponent; its sign goes into q, so that the largest product stays the
+    // largest score
+    const float scale = fmaxf(fabsf(a.scale_log2), 1e-30f);  // not 0: masked scores are -inf
+    const uint32_t sign = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+    auto flip = [&](uint4 x) { return make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign); };
     if (kPair || w == 0) {  // this thread's q row, K-major with the 128-byte swizzle
       const uint4* src = reinterpret_cast<const uint4*>(a.q + token * a.q_stride + (long)h * D);
       uint8_t* dst = sQ + (kPair ? w * C::kQ : 0) + t * 128;
 #pragma unroll
       for (int c = 0; c < D / 8; ++c)
         *reinterpret_cast<uint4*>(dst + (c >> 3) * (kRows * 128) + (((c & 7) ^ (t & 7)) << 4)) =
-            valid ? src[c] : make_uint4(0, 0, 0, 0);
+            valid ? flip(src[c]) : make_uint4(0, 0, 0, 0);
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_ready);
@@ -632,12 +648,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int limit =
         valid ? min(k1 - 1, seq_len(a, gr.first + tok / a.ql) - a.ql + tok % a.ql) : 0x7fffffff;  // padding: unmasked
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t tS = tmem + 128 * w + lanes, tO = tmem + 256 + 128 * w + lanes;
-    float m = kNegBig, l = 0.f;
+    const uint32_t tO = tmem + 256 + 128 * w + lanes;
+    float m = kNegBig, l = 0.f;  // m in the scaled log2 domain
     bool failed = false;
     const int n = count(w);
     for (int i = 0; i < n; ++i) {
-      if (!mbar_wait(&s_done[w], i & 1, abort_flag, a.status, kStatusAttnTimeout)) failed = true;
+      const uint32_t tS = tmem + 128 * w + 64 * (i & 1) + lanes;
+      if (!mbar_wait(&s_done[2 * w + (i & 1)], (i >> 1) & 1, abort_flag, a.status, kStatusAttnTimeout)) failed = true;
       if (__any_sync(0xffffffffu, failed)) {
         failed = true;
         break;
@@ -645,34 +662,32 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const int kv0 = k0 + tile(w, i) * kKv;
       if (any) {  // a warp of padding rows only signals
-        float v[8][16];
+        float v[4][16];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) tmem_ld_32x32b_x16(tS + 16 * c, v[c]);
+        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x16(tS + 16 * c, v[c]);
         tmem_wait_ld();
 #pragma unroll
-        for (int c = 0; c < 8; ++c) pin(v[c]);
-        float mx = kNegBig;
-        if (__all_sync(0xffffffffu, kv0 + kKv - 1 <= limit)) {
+        for (int c = 0; c < 4; ++c) pin(v[c]);
+        if (!__all_sync(0xffffffffu, kv0 + kKv - 1 <= limit)) {
 #pragma unroll
-          for (int c = 0; c < 8; ++c)
+          for (int c = 0; c < 4; ++c)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              v[c][e] *= a.scale_log2;
-              mx = fmaxf(mx, v[c][e]);
-            }
-        } else {
-#pragma unroll
-          for (int c = 0; c < 8; ++c)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              v[c][e] = kv0 + 16 * c + e <= limit ? v[c][e] * a.scale_log2 : -INFINITY;
-              mx = fmaxf(mx, v[c][e]);
-            }
+            for (int e = 0; e < 16; ++e) v[c][e] = kv0 + 16 * c + e <= limit ? v[c][e] : -INFINITY;
         }
-        const float m_new = fmaxf(m, mx);
+        float mx = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) mx = fmaxf(mx, v[c][e]);
+        const float m_new = fmaxf(m, mx == -INFINITY ? kNegBig : mx * scale);
         const bool grow = m_new > m + kLazy || i == 0;
         const float alpha = grow ? exp2f(m - m_new) : 1.f;
         if (i > 0 && __any_sync(0xffffffffu, grow)) {
+          const int j = i - 1;
+          if (!mbar_wait(&o_done[2 * w + (j & 1)], (j >> 1) & 1, abort_flag, a.status, kStatusAttnTimeout))
+            failed = true;
+          __syncwarp();
+          tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < D; c += 16) {
             float o[16];
@@ -691,12 +706,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {  // 32 keys -> 16 columns of P
+        for (int c = 0; c < 2; ++c) {  // 32 keys -> 16 columns of P
           uint32_t u[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const float p0 = exp2f(v[2 * c + (e >> 3)][(2 * e) & 15] - m);
-            const float p1 = exp2f(v[2 * c + (e >> 3)][(2 * e + 1) & 15] - m);
+            const float p0 = exp2f(fmaf(v[2 * c + (e >> 3)][(2 * e) & 15], scale, -m));
+            const float p1 = exp2f(fmaf(v[2 * c + (e >> 3)][(2 * e + 1) & 15], scale, -m));
             sum[e & 3] += p0 + p1;
             u[e] = pack_bf16x2(p0, p1);  // rounded by 2^-8 at most; l keeps the fp32 sum
           }
@@ -716,9 +731,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_ready[w]);
+      if (lane == 0) mbar_arrive(&p_ready[2 * w + (i & 1)]);
     }
-    if (!failed && n > 0 && !mbar_wait(&o_done[w], (n - 1) & 1, abort_flag, a.status, kStatusAttnTimeout)) failed = true;
+    if (!failed && n > 0 &&
+        !mbar_wait(&o_done[2 * w + ((n - 1) & 1)], ((n - 1) >> 1) & 1, abort_flag, a.status, kStatusAttnTimeout))
+      failed = true;
     failed = __any_sync(0xffffffffu, failed);
     if (!failed && any) {
       tc_fence_after();
@@ -755,15 +772,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // Each sequence's own keys, then the sum with the prefix.  grid (B, KV heads x row chunks, page splits), the splits of
 // a row one cluster.
-template <int D, int MT>
-__global__ void __launch_bounds__(kWarps * 32)
-    suffix_kernel(const __grid_constant__ CUtensorMap tm, const Args a, int row_chunks) {
-  extern __shared__ uint8_t raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  __shared__ int abort_flag;
-  if (threadIdx.x == 0) abort_flag = 0;
-  const int b = blockIdx.x, kh = blockIdx.y / row_chunks, r0 = blockIdx.y % row_chunks * (MT * 16);
-  const int G = a.nq / a.nkv, rows = min(MT * 16, a.ql * G - r0);
+template <int D, int NT>
+__global__ void __launch_bounds__(kWarps * 32, kCtas<D, NT>) suffix_kernel(const Args a, int row_chunks) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int b = blockIdx.x, kh = blockIdx.y / row_chunks, r0 = blockIdx.y % row_chunks * (NT * 8);
+  const int G = a.nq / a.nkv, rows = min(NT * 8, a.ql * G - r0);
   const int splits = gridDim.z, me = blockIdx.z;
   const Group gr = a.groups[a.seq_group[b]];
   const int len = seq_len(a, b);
@@ -771,7 +784,7 @@ __global__ void __launch_bounds__(kWarps * 32)
   const int begin = min(gr.prefix, len), p0 = begin / PAGE, pages = (len + PAGE - 1) / PAGE - p0;
   const int per = (pages + splits - 1) / splits;
   const int k0 = max(begin, (p0 + me * per) * PAGE), k1 = min(len, (p0 + (me + 1) * per) * PAGE);
-  float* res = stream<D, MT>(tm, a, smem, &abort_flag, a.table + (long)b * a.table_stride, kh, (long)b * a.ql, r0, rows,
+  float* res = stream<D, NT>(a, smem, a.table + (long)b * a.table_stride, kh, (long)b * a.ql, r0, rows,
                              min(k0, max(k1, 0)), k1, [&](int r) { return len - a.ql + (r0 + r) / G; });
   constexpr int RS = D + 2;
   cg::cluster_group cl = cg::this_cluster();
@@ -822,12 +835,12 @@ __global__ void __launch_bounds__(kWarps * 32)
   if (splits > 1) cl.sync();  // the others may still read this CTA's result
 }
 
-template <int D, int MT>
-void launch_prefix(const CUtensorMap& tm, const Args& a, int items, cudaStream_t stream) {
-  constexpr int smem = stream_smem<D, MT>();
+template <int D, int NT>
+void launch_prefix(const Args& a, int items, cudaStream_t stream) {
+  constexpr int smem = stream_smem<D, NT>(NT * 8);
   C10_CUDA_CHECK(
-      cudaFuncSetAttribute(prefix_stream_kernel<D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  prefix_stream_kernel<D, MT><<<dim3(items, a.nkv), kWarps * 32, smem, stream>>>(tm, a);
+      cudaFuncSetAttribute(prefix_stream_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  prefix_stream_kernel<D, NT><<<dim3(items, a.nkv), kWarps * 32, smem, stream>>>(a);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
@@ -840,11 +853,12 @@ void launch_prefix_tc(const CUtensorMap& tm, const Args& a, int items, cudaStrea
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
-template <int D, int MT>
-void launch_suffix(const CUtensorMap& tm, const Args& a, int splits, bool dependent, cudaStream_t stream) {
-  constexpr int smem = stream_smem<D, MT>();
-  C10_CUDA_CHECK(cudaFuncSetAttribute(suffix_kernel<D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  const int row_chunks = (a.ql * (a.nq / a.nkv) + MT * 16 - 1) / (MT * 16);
+template <int D, int NT>
+void launch_suffix(const Args& a, int splits, bool dependent, cudaStream_t stream) {
+  const int smem = stream_smem<D, NT>(std::min(NT * 8, a.ql * (a.nq / a.nkv)));
+  C10_CUDA_CHECK(cudaFuncSetAttribute(suffix_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      stream_smem<D, NT>(NT * 8)));
+  const int row_chunks = (a.ql * (a.nq / a.nkv) + NT * 8 - 1) / (NT * 8);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.B, a.nkv * row_chunks, splits);
   cfg.blockDim = dim3(kWarps * 32);
@@ -863,19 +877,22 @@ void launch_suffix(const CUtensorMap& tm, const Args& a, int splits, bool depend
   }
   cfg.attrs = at;
   cfg.numAttrs = n;
-  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, suffix_kernel<D, MT>, tm, a, row_chunks));
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, suffix_kernel<D, NT>, a, row_chunks));
 }
 
 template <int D>
 void run(const CUtensorMap& tm, const Args& a, int items, int tile_rows, int suffix_splits, cudaStream_t stream) {
   if (items > 0) {
-    if (tile_rows == 16) launch_prefix<D, 1>(tm, a, items, stream);
-    else if (tile_rows == 32) launch_prefix<D, 2>(tm, a, items, stream);
+    if (tile_rows == 8) launch_prefix<D, 1>(a, items, stream);
+    else if (tile_rows == 16) launch_prefix<D, 2>(a, items, stream);
+    else if (tile_rows == 32) launch_prefix<D, 4>(a, items, stream);
     else if (tile_rows == 128) launch_prefix_tc<D, false>(tm, a, items, stream);
     else launch_prefix_tc<D, true>(tm, a, items, stream);
   }
-  if (a.ql * (a.nq / a.nkv) <= 16) launch_suffix<D, 1>(tm, a, suffix_splits, items > 0, stream);
-  else launch_suffix<D, 2>(tm, a, suffix_splits, items > 0, stream);
+  const int rows = a.ql * (a.nq / a.nkv);
+  if (rows <= 8) launch_suffix<D, 1>(a, suffix_splits, items > 0, stream);
+  else if (rows <= 16) launch_suffix<D, 2>(a, suffix_splits, items > 0, stream);
+  else launch_suffix<D, 4>(a, suffix_splits, items > 0, stream);
 }
 
 }  // namespace shared_prefix
@@ -915,7 +932,7 @@ void shared_prefix_attention(const torch::Tensor& q, const torch::Tensor& kv_cac
                   groups.scalar_type() == at::kInt && groups.dim() == 2 && groups.size(1) == 4 &&
                   groups.is_contiguous(),
               "items and groups must be a plan's");
-  SP_CHECK(tile_rows == 16 || tile_rows == 32 || tile_rows == 128 || tile_rows == 256, "unknown row tile");
+  SP_CHECK(tile_rows == 8 || tile_rows == 16 || tile_rows == 32 || tile_rows == 128 || tile_rows == 256, "unknown row tile");
   SP_CHECK(suffix_splits == 1 || suffix_splits == 2 || suffix_splits == 4 || suffix_splits == 8, "suffix_splits must be 1, 2, 4 or 8");
   const uint64_t rows = (uint64_t)kv_cache.size(1) * 2 * nkv * PAGE;
   SP_CHECK(rows < (1ull << 31), "kv_cache has too many rows per layer for 32-bit tile coordinates");
@@ -954,6 +971,7 @@ void shared_prefix_attention(const torch::Tensor& q, const torch::Tensor& kv_cac
   a.part_o = ws.data_ptr<float>();
   a.part_ml = reinterpret_cast<float2*>(a.part_o + prefix_splits * T * nq * D);
   const auto* base = reinterpret_cast<const __nv_bfloat16*>(kv_cache.data_ptr()) + layer * kv_cache.stride(0);
+  a.kv = base;
   const CUtensorMap tm = make_tmap_bf16_2d(base, D, rows, D * 2, 64, PAGE);
   if (D == 128) run<128>(tm, a, int(items.size(0)), int(tile_rows), int(suffix_splits), stream);
   else run<64>(tm, a, int(items.size(0)), int(tile_rows), int(suffix_splits), stream);

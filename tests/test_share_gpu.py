@@ -142,8 +142,9 @@ def test_strides_and_layer():
 
 
 @pytest.mark.parametrize("scale", [1.0, -0.3, 0.0, 8.0])
-def test_scales(scale):
-    b = Batch((8, 2, 128), [5], [150], [1, 30])
+@pytest.mark.parametrize("members", [5, 20, 40])
+def test_scales(scale, members):
+    b = Batch((8, 2, 128), [members], [150], [1, 30])
     b.scale = scale
     b.check(b.run())
 
