@@ -554,7 +554,7 @@ class SharedPrefixPlan:
     and their prefixes alone, so a serving loop keeps it over all layers and steps (and graph replays) until a
     member is added.  Members that end keep their place with length 0.  Nothing in it changes after it is made."""
 
-    __slots__ = ("items", "groups", "seq_group", "tile_rows", "prefix_splits", "suffix_splits", "batch", "num_q_heads",
+    __slots__ = ("items", "groups", "seqs", "tile_rows", "prefix_splits", "suffix_splits", "batch", "num_q_heads",
                  "num_kv_heads", "head_dim", "q_len")
 
 
@@ -600,26 +600,27 @@ def shared_prefix_plan(group_sizes, prefix_lens, *, num_q_heads: int, num_kv_hea
     tiles = [-(-r // p.tile_rows) for r in rows]
     step, slots = (64, 2 * sms) if p.tile_rows <= 32 else (128 if p.tile_rows == 256 else 256, sms)
     chunk = _prefix_chunk(prefix, [t * num_kv_heads for t in tiles], step, slots)
-    items, groups, seq_group = [], [], []
+    items, groups, seqs = [], [], []
     p.prefix_splits = 1
     first = 0
     for g, (n, pre) in enumerate(zip(sizes, prefix)):
         splits = -(-pre // chunk)
         p.prefix_splits = max(p.prefix_splits, splits)
         groups.append((first, n, pre, chunk))
-        seq_group += [g] * n
+        seqs += [(pre, splits)] * n
         items += [(g, t * p.tile_rows, s, 0) for s in range(splits) for t in range(tiles[g])]
         first += n
     p.batch, p.num_q_heads, p.num_kv_heads, p.head_dim, p.q_len = first, num_q_heads, num_kv_heads, head_dim, q_len
-    # a sequence's own pages: one CTA per KV head and 32 rows, split while CTAs are few and pages many
+    # A sequence's own pages: one CTA of up to 8 warps per KV head and 32 rows, and where those are too few for the
+    # SMs and the pages many, a cluster of them.
     own = (max_seq_len - min(prefix, default=0)) if max_seq_len is not None else 1024
     ctas = first * num_kv_heads * (-(-per_seq // 32))
     p.suffix_splits = 1
-    while p.suffix_splits < 8 and ctas * p.suffix_splits < 2 * sms and own // p.suffix_splits >= 256:
+    while p.suffix_splits < 8 and ctas * p.suffix_splits * 2 <= sms and own // p.suffix_splits >= 512:
         p.suffix_splits *= 2
     p.items = torch.tensor(items, dtype=torch.int32).view(-1, 4).to(device)
     p.groups = torch.tensor(groups, dtype=torch.int32).view(-1, 4).to(device)
-    p.seq_group = torch.tensor(seq_group, dtype=torch.int32).to(device)
+    p.seqs = torch.tensor(seqs, dtype=torch.int32).view(-1, 2).to(device)
     return p
 
 
@@ -636,7 +637,7 @@ def shared_prefix_attention(q, kv_cache, layer, block_table, seq_lens, out, *, p
             (kv_cache.dim() == 6 and kv_cache.shape[3] != plan.num_kv_heads):
         raise ValueError("shared_prefix_attention: the plan was made for other heads")
     _C().shared_prefix_attention(q, kv_cache, layer, block_table, seq_lens, out, plan.items, plan.groups,
-                                 plan.seq_group, plan.q_len, plan.tile_rows, plan.prefix_splits, plan.suffix_splits,
+                                 plan.seqs, plan.q_len, plan.tile_rows, plan.prefix_splits, plan.suffix_splits,
                                  scale)
     _count(2 if plan.items.shape[0] else 1)
     return out

@@ -9,11 +9,11 @@ namespace bloom {
 // capture, where it would become part of the graph (zeroed by every replay).  (csrc/kernels/sampling.cu)
 int* status_word(int64_t device);
 
-// Decode / verify attention with group-shared prefixes (shared_prefix.cu); items, groups, seq_group, tile_rows and
+// Decode / verify attention with group-shared prefixes (shared_prefix.cu); items, groups, seqs, tile_rows and
 // prefix_splits are those of one plan (ops.shared_prefix_plan).
 void shared_prefix_attention(const torch::Tensor& q, const torch::Tensor& kv_cache, int64_t layer,
                              const torch::Tensor& block_table, const torch::Tensor& seq_lens, torch::Tensor& out,
-                             const torch::Tensor& items, const torch::Tensor& groups, const torch::Tensor& seq_group,
+                             const torch::Tensor& items, const torch::Tensor& groups, const torch::Tensor& seqs,
                              int64_t q_len, int64_t tile_rows, int64_t prefix_splits, int64_t suffix_splits,
                              double scale);
 

@@ -32,17 +32,14 @@ namespace shared_prefix {
 
 constexpr int PAGE = 16;
 constexpr float kNegBig = -1e30f;
-constexpr int kWarps = 4;  // of a streaming CTA
-// CTAs per SM that the registers are kept low enough for: O alone takes NT * D / 4 of them
-template <int D, int NT>
-constexpr int kCtas = D * NT >= 512 ? 2 : D * NT >= 256 ? 3 : 4;
+constexpr int kStages = 3;   // ring depth of a streaming warp, in pages
+constexpr int kMaxWarps = 8; // of a streaming CTA: 8 rings fill an SM's shared memory (and 255 registers its file)
 
 struct Group {  // one row of plan.groups
   int first, members, prefix, chunk;  // first sequence, sequences, shared tokens, prefix tokens per split
 };
 
 struct Args {
-  const __nv_bfloat16* kv; // this layer's pages [NB, 2, nkv, 16, D]
   const __nv_bfloat16* q;  // [B * ql, nq, D]
   long q_stride;           // elements between token rows
   __nv_bfloat16* out;
@@ -53,15 +50,30 @@ struct Args {
   const int* lens;         // [B]
   const int4* items;       // prefix work: {group, first row, split, -}
   const Group* groups;
-  const int* seq_group;    // [B]
+  const int2* seqs;        // [B] {shared tokens, splits of them}
   float* part_o;           // [splits, B * ql, nq, D]
   float2* part_ml;         // [splits, B * ql, nq]
   int B, nq, nkv, ql, NB;
   int parts;               // partial sums per prefix split: 2 where the two streams of a CTA leave one each
+  uint32_t per_g;          // ceil(2^32 / G), G = nq / nkv: r / G = (r * per_g) >> 32 while r * G < 2^32
   float scale_log2;
   int* status;
 };
 
+__device__ __forceinline__ int div_g(const Args& a, int r) {
+  return a.per_g ? int(__umulhi(unsigned(r), a.per_g)) : r;  // 0 stands for 2^32: G = 1
+}
+
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+               : "r"(addr));
+}
 __device__ __forceinline__ void mma_bf16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
@@ -70,6 +82,12 @@ __device__ __forceinline__ void mma_bf16_16816(float (&d)[4], const uint32_t (&a
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Byte address of element (tok, d), d a multiple of 8, of a page that TMA wrote as 2 KB boxes of 64 dims with the
+// 128-byte swizzle.
+__device__ __forceinline__ uint32_t page_addr(uint32_t base, int tok, int d) {
+  return base + ((d >> 6) << 11) + (tok << 7) + (((((d & 63) >> 3) ^ (tok & 7))) << 4);
+}
 
 // Length of sequence b, kept inside its table row.
 __device__ __forceinline__ int seq_len(const Args& a, int b) {
@@ -106,14 +124,13 @@ __device__ __forceinline__ int2 prefix_holder(const Args& a, const Group& g) {
   return make_int2(g.first + int(0xffffffffu - unsigned(best)), int(best >> 32));
 }
 
-// Shared memory of a streaming CTA: the query rows (where they do not stay in registers), and one partial result per
-// warp and row.
 template <int D>
-constexpr int kQStride = D * 2 + 64;  // bytes of a query row: neighbouring rows start in different banks
-template <int D, int NT>
-constexpr int q_bytes() { return NT > 1 ? NT * 8 * kQStride<D> : 0; }
-template <int D, int NT>
-constexpr int stream_smem(int rows) { return q_bytes<D, NT>() + kWarps * rows * (D + 2) * 4; }
+constexpr int stage_bytes() { return 2 * PAGE * D * 2; }  // a page's K and V
+// Shared memory of a streaming CTA: the warps' rings, after the loop one partial result per warp and row; barriers.
+template <int D>
+int stream_smem(int warps, int rows) {
+  return std::max(warps * kStages * stage_bytes<D>(), warps * rows * (D + 2) * 4) + warps * kStages * 8 + 1024;
+}
 
 // Streams keys [k_begin, k_end) of one KV head past up to NT * 8 packed query rows (row r: token q0 + (r0 + r) / G,
 // q head kh * G + (r0 + r) % G; limit(r): the last key that it sees) and leaves, in shared memory, row r's O[D], m, l at
@@ -121,74 +138,62 @@ constexpr int stream_smem(int rows) { return q_bytes<D, NT>() + kWarps * rows * 
 //
 // The products are formed transposed, S^T = K Q^T and O^T = V^T P^T, so that keys and dims fill the 16-row side of
 // m16n8k16 and 4 to 8 query rows (a GQA group) fill its 8-column side: half the MMAs and half the registers for O of
-// the other way round.  Each warp takes every kWarps-th page and loads it straight into A fragments, 16 bytes a load:
-// the dims of Q K^T may be summed in any order, so a thread's 8 contiguous dims of a key are fragments of two MMAs (Q in
-// the same order); for P V the 8 contiguous dims of 4 keys are interleaved by byte permutes.  P^T moves from
-// accumulator to B fragments by an 8x8 transpose of the warp.  The next page's K is requested once S is formed, its V
-// once P V is issued: 8 KB in flight per warp without shared memory, barriers or ldmatrix.
+// the other way round.  P^T moves from accumulator to B fragments by an 8x8 transpose of the warp.  Each warp takes
+// every warps-th page through its own TMA ring.  (Loading fragments straight into registers needs no barriers, but
+// keeps only a page per warp in flight, and at 128 registers spills: 79 us where the rings take XX us for 268 MB of
+// 2,048 short sequences x heads.)
 template <int D, int NT, typename Limit>
-__device__ float* stream(const Args& a, uint8_t* smem, const int* row, int kh, long q0, int r0, int rows, int k_begin,
-                         int k_end, Limit&& limit_of) {
-  constexpr int RS = D + 2, NC = D / 32, NB = D / 64;
-  const int warp = warp_id(), lane = lane_id(), g = lane >> 2, t4 = lane & 3;
+__device__ float* stream(const CUtensorMap& tm, const Args& a, uint8_t* smem, int* abort_flag, const int* row, int kh,
+                         long q0, int r0, int rows, int k_begin, int k_end, Limit&& limit_of) {
+  constexpr int RS = D + 2, kStage = stage_bytes<D>(), kPageB = PAGE * D * 2;
+  const int warps = blockDim.x / 32, warp = warp_id(), lane = lane_id(), g = lane >> 2, t4 = lane & 3;
   const int G = a.nq / a.nkv;
   const int p0 = k_begin / PAGE, p1 = k_end > k_begin ? (k_end + PAGE - 1) / PAGE : p0;
   const int first = p0 + warp;
-  const int n = p1 > first ? (p1 - first + kWarps - 1) / kWarps : 0;
+  const int n = p1 > first ? (p1 - first + warps - 1) / warps : 0;
+  uint8_t* ring = smem + warp * kStages * kStage;
+  uint64_t* bars =
+      reinterpret_cast<uint64_t*>(smem + max(warps * kStages * kStage, warps * rows * RS * 4)) + warp * kStages;
 
   int ids = 0;  // block ids of this warp's next 32 pages, one per lane
   auto fetch_ids = [&](int i) {
-    const int p = first + (i + lane) * kWarps;
+    const int p = first + (i + lane) * warps;
     ids = p < p1 ? block_id(a, row, p) : 0;
   };
-  auto page_of = [&](int i, int kv) {
-    const long blk = __shfl_sync(0xffffffffu, ids, i & 31);
-    return a.kv + ((blk * 2 + kv) * a.nkv + kh) * (PAGE * D);
-  };
-  uint4 kf[2][NC], vf[4][NB];
-  auto load_k = [&](int i) {  // keys g and g + 8
-    const __nv_bfloat16* p = page_of(i, 0) + g * D + t4 * 8;
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int c = 0; c < NC; ++c) kf[h][c] = __ldg(reinterpret_cast<const uint4*>(p + h * 8 * D + c * 32));
-  };
-  auto load_v = [&](int i) {  // keys 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9 of the page
-    const __nv_bfloat16* p = page_of(i, 1) + 2 * t4 * D + g * 8;
-    const int left = k_end - (first + i * kWarps) * PAGE;  // slots at or behind the last key may hold anything: zeros
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int tok = (k & 1) + 8 * (k >> 1);
-#pragma unroll
-      for (int d = 0; d < NB; ++d)
-        vf[k][d] = 2 * t4 + tok < left ? __ldg(reinterpret_cast<const uint4*>(p + tok * D + d * 64))
-                                       : make_uint4(0, 0, 0, 0);
+  auto issue = [&](int i) {
+    if ((i & 31) == 0) fetch_ids(i);
+    const int blk = __shfl_sync(0xffffffffu, ids, i & 31), s = i % kStages;
+    if (lane == 0) {
+      const int rowK = (blk * 2 * a.nkv + kh) * PAGE, rowV = rowK + a.nkv * PAGE;
+      uint8_t* st = ring + s * kStage;
+      mbar_arrive_expect_tx(&bars[s], kStage);
+      tma_load_2d(st, &tm, &bars[s], 0, rowK);
+      if constexpr (D == 128) tma_load_2d(st + 2048, &tm, &bars[s], 64, rowK);
+      tma_load_2d(st + kPageB, &tm, &bars[s], 0, rowV);
+      if constexpr (D == 128) tma_load_2d(st + kPageB + 2048, &tm, &bars[s], 64, rowV);
     }
   };
-  if (n > 0) {
-    fetch_ids(0);
-    load_k(0);
-    load_v(0);
+  if (lane == 0) {  // a ring belongs to its warp: no other thread waits on it
+    for (int s = 0; s < kStages; ++s) mbar_init(&bars[s], 1);
+    fence_barrier_init();
   }
-  // Q^T fragments: row g of each 8-row tile, this thread's 8 dims of each 32
-  auto q_row = [&](int r) { return a.q + (q0 + (r0 + r) / G) * a.q_stride + (kh * G + (r0 + r) % G) * D; };
-  uint4 qr[NC];
-  if constexpr (NT == 1) {
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-      qr[c] = g < rows ? __ldg(reinterpret_cast<const uint4*>(q_row(g) + c * 32 + t4 * 8)) : make_uint4(0, 0, 0, 0);
-  } else {
-    for (int c = threadIdx.x; c < NT * 8 * (D / 8); c += kWarps * 32) {
-      const int r = c / (D / 8), d = c % (D / 8);
-      *reinterpret_cast<uint4*>(smem + r * kQStride<D> + d * 16) =
-          r < rows ? __ldg(reinterpret_cast<const uint4*>(q_row(r) + d * 8)) : make_uint4(0, 0, 0, 0);
-    }
-    __syncthreads();
-  }
+  __syncwarp();
+  for (int i = 0; i < kStages && i < n; ++i) issue(i);
+
+  // Q^T fragments: row g of each 8-row tile, dims 16 ks + 2 t4 and the next, + 8
+  uint32_t qf[NT][D / 16][2];
   int limit[NT][2], low = 0x7fffffff;  // of rows 8 nt + 2 t4 + e
   float m_run[NT][2], l_run[NT][2], o[NT][D / 16][4];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
+    const int rq = nt * 8 + g, qi = div_g(a, r0 + rq);
+    const uint32_t* q =
+        reinterpret_cast<const uint32_t*>(a.q + (q0 + qi) * a.q_stride + (kh * G + r0 + rq - qi * G) * D) + t4;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      qf[nt][ks][0] = rq < rows ? __ldg(q + 8 * ks) : 0u;
+      qf[nt][ks][1] = rq < rows ? __ldg(q + 8 * ks + 4) : 0u;
+    }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int r = nt * 8 + 2 * t4 + e;
@@ -201,27 +206,31 @@ __device__ float* stream(const Args& a, uint8_t* smem, const int* row, int kh, l
     for (int j = 0; j < D / 16; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
   }
   low = __reduce_min_sync(0xffffffffu, low);
-  for (int i = 0; i < n; ++i) {
-    const int tok0 = (first + i * kWarps) * PAGE;
+  bool ok = true;
+  int i = 0;
+  for (; i < n; ++i) {
+    const int s = i % kStages;
+    ok = __all_sync(0xffffffffu, mbar_wait(&bars[s], (i / kStages) & 1, abort_flag, a.status, kStatusAttnTimeout));
+    if (!ok) break;
+    const uint32_t sK = smem_u32(ring + s * kStage), sV = sK + kPageB;
+    const int tok0 = (first + i * warps) * PAGE;
+    if (tok0 + PAGE > k_end) {  // V rows behind the last key: whatever they hold must not meet p = 0
+      for (int c = lane; c < PAGE * D / 8; c += 32) {
+        const int tok = c & 15, d = (c >> 4) * 8;
+        if (tok0 + tok >= k_end)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(page_addr(sV, tok, d)), "r"(0) : "memory");
+      }
+      __syncwarp();
+    }
     float sc[NT][4];  // [key g: rows 2 t4, 2 t4 + 1 | key g + 8: the same]
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const uint32_t a0[4] = {kf[0][c].x, kf[1][c].x, kf[0][c].y, kf[1][c].y};
-      const uint32_t a1[4] = {kf[0][c].z, kf[1][c].z, kf[0][c].w, kf[1][c].w};
+    for (int ks = 0; ks < D / 16; ++ks) {
+      uint32_t k[4];
+      ldsm_x4(page_addr(sK, lane & 15, 16 * ks + 8 * (lane >> 4)), k[0], k[1], k[2], k[3]);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        uint4 q;
-        if constexpr (NT == 1) q = qr[c];
-        else q = *reinterpret_cast<const uint4*>(smem + (nt * 8 + g) * kQStride<D> + c * 64 + t4 * 16);
-        mma_bf16_16816(sc[nt], a0, q.x, q.y);
-        mma_bf16_16816(sc[nt], a1, q.z, q.w);
-      }
-    }
-    if (i + 1 < n) {
-      if (((i + 1) & 31) == 0) fetch_ids(i + 1);
-      load_k(i + 1);
+      for (int nt = 0; nt < NT; ++nt) mma_bf16_16816(sc[nt], k, qf[nt][ks][0], qf[nt][ks][1]);
     }
     const bool whole = tok0 >= k_begin && tok0 + PAGE - 1 <= low;  // every row sees every key of the page
     uint32_t pb[NT][2];
@@ -270,20 +279,24 @@ __device__ float* stream(const Args& a, uint8_t* smem, const int* row, int kh, l
       }
     }
 #pragma unroll
-    for (int d = 0; d < NB; ++d)
+    for (int j = 0; j < D / 16; ++j) {  // dims 16 j + g and + 8
+      uint32_t v[4];
+      ldsm_x4_t(page_addr(sV, (lane & 7) + 8 * (lane >> 4), 16 * j + (lane & 8)), v[0], v[1], v[2], v[3]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {  // rows g and g + 8 of tile j are dims 64 d + 8 g + 2 j and the next
-        auto word = [&](const uint4& v) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; };
-        const uint32_t w0 = word(vf[0][d]), w1 = word(vf[1][d]), w2 = word(vf[2][d]), w3 = word(vf[3][d]);
-        const uint32_t av[4] = {__byte_perm(w0, w1, 0x5410), __byte_perm(w0, w1, 0x7632), __byte_perm(w2, w3, 0x5410),
-                                __byte_perm(w2, w3, 0x7632)};
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma_bf16_16816(o[nt][4 * d + j], av, pb[nt][0], pb[nt][1]);
-      }
-    if (i + 1 < n) load_v(i + 1);
+      for (int nt = 0; nt < NT; ++nt) mma_bf16_16816(o[nt][j], v, pb[nt][0], pb[nt][1]);
+    }
+    __syncwarp();
+    if (i + kStages < n) {
+      if (lane == 0) fence_proxy_async();
+      issue(i + kStages);
+    }
   }
-  // the warps' results into shared memory, then summed into warp 0's place
-  float* cm = reinterpret_cast<float*>(smem + q_bytes<D, NT>());
+  if (!ok && lane == 0)  // gave up: the loads in flight must land before the shared memory is reused
+    for (int k = i; k < n && k < i + kStages; ++k) mbar_drain(&bars[k % kStages], (k / kStages) & 1);
+  if (warps > 1) __syncthreads();
+  else __syncwarp();
+  // the warps' results over their rings, then summed into warp 0's place
+  float* cm = reinterpret_cast<float*>(smem);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -295,36 +308,34 @@ __device__ float* stream(const Args& a, uint8_t* smem, const int* row, int kh, l
       if (r < rows) {
         float* w = cm + (warp * rows + r) * RS;
 #pragma unroll
-        for (int d = 0; d < NB; ++d)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<float2*>(w + 64 * d + 8 * g + 2 * j) =
-                make_float2(o[nt][4 * d + j][e], o[nt][4 * d + j][2 + e]);
+        for (int j = 0; j < D / 16; ++j) {
+          w[16 * j + g] = o[nt][j][e];
+          w[16 * j + 8 + g] = o[nt][j][2 + e];
+        }
         if (g == 0) *reinterpret_cast<float2*>(w + D) = make_float2(m_run[nt][e], l);
       }
     }
+  if (warps == 1) {
+    __syncwarp();
+    return cm;
+  }
   __syncthreads();
-  // one warp per row: every lane reads the row's (m, l) of all warps before any lane writes the sums back
-  for (int r = warp; r < rows; r += kWarps) {
-    float m[kWarps], M = kNegBig, L = 0.f;
+  // one warp per row, the (m, l) of part w in lane w
+  for (int r = warp; r < rows; r += warps) {
+    const float2 ml = lane < warps ? *reinterpret_cast<const float2*>(cm + (lane * rows + r) * RS + D)
+                                   : make_float2(kNegBig, 0.f);
+    const float M = warp_max(ml.x), f = exp2f(ml.x - M), L = warp_sum(ml.y * f);
+    float O[D / 32];
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      m[w] = cm[(w * rows + r) * RS + D];
-      M = fmaxf(M, m[w]);
-    }
+    for (int c = 0; c < D / 32; ++c) O[c] = 0.f;
+    for (int w = 0; w < warps; ++w) {
+      const float fw = __shfl_sync(0xffffffffu, f, w);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      m[w] = exp2f(m[w] - M);
-      L += cm[(w * rows + r) * RS + D + 1] * m[w];
+      for (int c = 0; c < D / 32; ++c) O[c] += cm[(w * rows + r) * RS + c * 32 + lane] * fw;
     }
     __syncwarp();
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c) {
-      float O = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) O += cm[(w * rows + r) * RS + c * 32 + lane] * m[w];
-      cm[r * RS + c * 32 + lane] = O;
-    }
+    for (int c = 0; c < D / 32; ++c) cm[r * RS + c * 32 + lane] = O[c];
     if (lane == 0) *reinterpret_cast<float2*>(cm + r * RS + D) = make_float2(M, L);
   }
   __syncthreads();
@@ -333,9 +344,14 @@ __device__ float* stream(const Args& a, uint8_t* smem, const int* row, int kh, l
 
 // Prefix work of groups with few rows: the keys stream past at most NT * 8 of them.  grid (items, KV heads).
 template <int D, int NT>
-__global__ void __launch_bounds__(kWarps * 32, kCtas<D, NT>) prefix_stream_kernel(const Args a) {
+__global__ void __launch_bounds__(kMaxWarps * 32) 
+    prefix_stream_kernel(const __grid_constant__ CUtensorMap tm, const Args a) {
   griddep_launch_dependents();
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  __shared__ int abort_flag;
+  if (threadIdx.x == 0) abort_flag = 0;
+  __syncthreads();
   const int4 it = a.items[blockIdx.x];
   const Group gr = a.groups[it.x];
   const int kh = blockIdx.y, G = a.nq / a.nkv;
@@ -343,14 +359,14 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, NT>) prefix_stream_kerne
   const int k0 = min(it.z * gr.chunk, hold.y), k1 = min(k0 + gr.chunk, hold.y);
   const int rows = min(NT * 8, gr.members * a.ql * G - it.y);
   const long q0 = (long)gr.first * a.ql;
-  const float* res = stream<D, NT>(a, smem, a.table + hold.x * a.table_stride, kh, q0, it.y, rows, k0, k1, [&](int r) {
-                                     const int tok = (it.y + r) / G;
+  const float* res = stream<D, NT>(tm, a, smem, &abort_flag, a.table + hold.x * a.table_stride, kh, q0, it.y, rows, k0, k1, [&](int r) {
+                                     const int tok = div_g(a, it.y + r);
                                      return seq_len(a, gr.first + tok / a.ql) - a.ql + tok % a.ql;
                                    });
   constexpr int RS = D + 2;
-  for (int idx = threadIdx.x; idx < rows * (D / 4); idx += kWarps * 32) {
+  for (int idx = threadIdx.x; idx < rows * (D / 4); idx += blockDim.x) {
     const int r = idx / (D / 4), d = idx % (D / 4) * 4;
-    const long at = ((long)it.z * a.B * a.ql + q0 + (it.y + r) / G) * a.nq + kh * G + (it.y + r) % G;
+    const long at = ((long)it.z * a.B * a.ql + q0 + div_g(a, it.y + r)) * a.nq + kh * G + (it.y + r - div_g(a, it.y + r) * G);
     const float* p = res + r * RS + d;
     *reinterpret_cast<float4*>(a.part_o + at * D + d) = make_float4(p[0], p[1], p[2], p[3]);
     if (d == 0) a.part_ml[at] = make_float2(res[r * RS + D], res[r * RS + D + 1]);
@@ -368,12 +384,11 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, NT>) prefix_stream_kerne
 // per stream, S(i + 1) had to wait for P V(i), and each tile's softmax for both: 6,300 cycles per 128 keys of a pair,
 // half of them waiting.  The running max is lazy: O is rescaled (and P V(i - 1) waited for) only when a row's max
 // grows by more than 2^8.
-// Warps 0-7 softmax and epilogue, warp 8 TMA producer and TMEM owner, warp 9 issues the MMAs of both streams from an
-// event loop over their barriers.
+// Warps 0-7 softmax and epilogue, warp 8 TMA producer and TMEM owner, warps 9 and 10 issue the MMAs of a stream each.
 namespace tc {
 
 constexpr int kRows = 128, kKv = 64;
-constexpr int kThreads = 256 + 64;
+constexpr int kThreads = 256 + 32 + 64;
 constexpr int kTmemCols = 512;
 constexpr float kLazy = 8.f;  // log2 units
 
@@ -444,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // [2 * stream + (tile & 1)]
   uint64_t *s_done = bars + 32, *p_ready = bars + 36, *o_done = bars + 40;
   uint64_t *q_ready = bars + 44, *drain = bars + 45;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 46);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 47);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = warp_id(), lane = lane_id();
@@ -474,7 +489,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&o_done[w], 1);
     }
     mbar_init(q_ready, kPair ? 8 : 4);
-    mbar_init(drain, 1);
+    mbar_init(&drain[0], 1);
+    mbar_init(&drain[1], 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -541,94 +557,73 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int j = max(0, nK - kStages); j < nK; ++j) mbar_drain(&fullK[j % kStages], (j / kStages) & 1);
       for (int j = max(0, nV - kStages); j < nV; ++j) mbar_drain(&fullV[j % kStages], (j / kStages) & 1);
     }
-  } else if (warp == 9) {
-    // The whole warp runs the loop and one elected lane issues: operands of tcgen05.mma live in uniform registers, and
-    // in a branch on the lane every one of them is moved there for every instruction (90 cycles an MMA for S, 300 for
-    // P V, so that issuing took three times as long as the tensor pipe's work).  Answers of barriers are broadcast,
-    // which keeps the loop's state uniform.
-    if (n_kt > 0) {
-      auto done = [&](uint64_t* bar, uint32_t parity) {
-        return __shfl_sync(0xffffffffu, int(mbar_test(bar, parity)), 0) != 0;
-      };
-      constexpr uint32_t idS = umma_idesc_bf16(kRows, kKv);
-      constexpr uint32_t idO = umma_idesc_bf16(kRows, D) | (1u << 16);  // B is MN-major
-      bool issued = false;
-      bool ok = __shfl_sync(0xffffffffu, int(mbar_wait(q_ready, 0, abort_flag, a.status, kStatusAttnTimeout)), 0) != 0;
-      // per stream: the next tile whose S, and whose P V, is to be issued
-      int iS[2] = {0, 0}, iP[2] = {0, 0};
-      int left = (count(0) > 0) + (count(1) > 0);
-      uint64_t t_stall = 0;
-      uint32_t spins = 0;  // since the last progress
-      while (ok && left > 0) {
-        bool progressed = false;
+  } else if (warp >= 9) {
+    // One warp per stream issues its MMAs.  The whole warp runs the loop and one elected lane issues: operands of
+    // tcgen05.mma live in uniform registers, and in a branch on the lane every one of them is moved there for every
+    // instruction (90 cycles an MMA for S, 300 for P V: three times the tensor pipe's own work).  One warp for both
+    // streams, polling their barriers in turn, spent as long on the polls as on issuing.
+    const int w = warp - 9, n = count(w);
+    constexpr uint32_t idS = umma_idesc_bf16(kRows, kKv);
+    constexpr uint32_t idO = umma_idesc_bf16(kRows, D) | (1u << 16);  // B is MN-major
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, a.status, kStatusAttnTimeout)) != 0;
+    };
+    auto issue_s = [&](int i) {
+      const int t = tile(w, i), s = t % kStages;
+      // the S buffer is free once P V of the tile two back has read P from it
+      if (!wait(&fullK[s], (t / kStages) & 1) || (i >= 2 && !wait(&o_done[2 * w + (i & 1)], ((i >> 1) - 1) & 1)))
+        return false;
+      tc_fence_after();
+      const uint64_t dq = umma_desc_sw128(smem_u32(sQ + (kPair ? w * C::kQ : 0)));
+      const uint64_t dk = umma_desc_sw128(smem_u32(sK + s * C::kTile));
+      if (elect_one_sync()) {
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const int i = iS[w], t = tile(w, i), s = t % kStages;
-          // the S buffer is free once P V of the tile two back has read P from it
-          if (i < count(w) && done(&fullK[s], (t / kStages) & 1) &&
-              (i < 2 || done(&o_done[2 * w + (i & 1)], ((i >> 1) - 1) & 1))) {
-            tc_fence_after();
-            const uint32_t kb = smem_u32(sK + s * C::kTile), qb = smem_u32(sQ + (kPair ? w * C::kQ : 0));
-            const uint64_t dq = umma_desc_sw128(qb), dk = umma_desc_sw128(kb);
-            if (elect_one_sync()) {
-#pragma unroll
-              for (int kk = 0; kk < D / 16; ++kk)  // descriptors count addresses in 16 bytes
-                umma_f16(tmem + 128 * w + 64 * (i & 1), dq + (kk >> 2) * (kRows * 8) + 2 * (kk & 3),
-                         dk + (kk >> 2) * (C::kRegion / 16) + 2 * (kk & 3), idS, kk > 0 ? 1u : 0u);
-              umma_commit(&s_done[2 * w + (i & 1)]);
-              umma_commit(&emptyK[s]);
-            }
-            __syncwarp();
-            ++iS[w];
-            issued = progressed = true;
-          }
-          const int j = iP[w], tv = tile(w, j), sv = tv % kStages;
-          if (j < iS[w] && done(&p_ready[2 * w + (j & 1)], (j >> 1) & 1) && done(&fullV[sv], (tv / kStages) & 1)) {
-            tc_fence_after();
-            const uint64_t dv = desc_mn(smem_u32(sV + sv * C::kTile), C::kRegion);
-            if (elect_one_sync()) {
-#pragma unroll
-              for (int kk = 0; kk < kKv / 16; ++kk)
-                umma_f16_ts(tmem + 256 + 128 * w, tmem + 128 * w + 64 * (j & 1) + 8 * kk, dv + kk * (16 * 128 / 16), idO,
-                            (j > 0 || kk > 0) ? 1u : 0u);
-              umma_commit(&o_done[2 * w + (j & 1)]);
-              umma_commit(&emptyV[sv]);
-            }
-            __syncwarp();
-            if (++iP[w] == count(w)) --left;
-            progressed = true;
-          }
-        }
-        if (progressed) {
-          spins = 0;
-        } else if ((++spins & 63u) == 0) {
-          bool stop = false;
-          if (lane == 0) {
-            stop = *abort_flag;
-            if (spins == 64) t_stall = globaltimer_ns();
-            if (!stop && globaltimer_ns() - t_stall > kLocalWaitTimeoutNs) {
-              *abort_flag = 1;
-              atomicOr(a.status, kStatusAttnTimeout);
-              stop = true;
-            }
-          }
-          ok = !__shfl_sync(0xffffffffu, int(stop), 0);
-        }
+        for (int kk = 0; kk < D / 16; ++kk)  // descriptors count addresses in 16 bytes
+          umma_f16(tmem + 128 * w + 64 * (i & 1), dq + (kk >> 2) * (kRows * 8) + 2 * (kk & 3),
+                   dk + (kk >> 2) * (C::kRegion / 16) + 2 * (kk & 3), idS, kk > 0 ? 1u : 0u);
+        umma_commit(&s_done[2 * w + (i & 1)]);
+        umma_commit(&emptyK[s]);
       }
-      if (!ok && issued) {  // what was issued completes before TMEM is freed
-        if (elect_one_sync()) umma_commit(drain);
-        __syncwarp();
-        mbar_drain(drain, 0);
+      __syncwarp();
+      return true;
+    };
+    bool ok = n > 0 && wait(q_ready, 0) && issue_s(0);
+    bool issued = ok;
+    for (int i = 0; i < n && ok; ++i) {
+      if (i + 1 < n && !issue_s(i + 1)) {
+        ok = false;
+        break;
       }
+      const int t = tile(w, i), s = t % kStages;
+      if (!wait(&p_ready[2 * w + (i & 1)], (i >> 1) & 1) || !wait(&fullV[s], (t / kStages) & 1)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint64_t dv = desc_mn(smem_u32(sV + s * C::kTile), C::kRegion);
+      if (elect_one_sync()) {
+#pragma unroll
+        for (int kk = 0; kk < kKv / 16; ++kk)
+          umma_f16_ts(tmem + 256 + 128 * w, tmem + 128 * w + 64 * (i & 1) + 8 * kk, dv + kk * (16 * 128 / 16), idO,
+                      (i > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(&o_done[2 * w + (i & 1)]);
+        umma_commit(&emptyV[s]);
+      }
+      __syncwarp();
+    }
+    if (!ok && issued) {  // what was issued completes before TMEM is freed
+      if (elect_one_sync()) umma_commit(&drain[w]);
+      __syncwarp();
+      mbar_drain(&drain[w], 0);
     }
   } else {
     const int w = warp >> 2, t = threadIdx.x & (kRows - 1);
     const int r = it.y + (kPair ? w * kRows : 0) + t;
     const bool valid = r < rows;
     const bool any = __any_sync(0xffffffffu, valid);
-    const int tok = (valid ? r : 0) / G;
+    const int tok = div_g(a, valid ? r : 0);
     const long token = (long)gr.first * a.ql + tok;
-    const int h = kh * G + (valid ? r : 0) % G;
+    const int h = kh * G + (valid ? r : 0) - tok * G;
     // scores are scaled by |scale| inside the exponent; its sign goes into q, so that the largest product stays the
     // largest score
     const float scale = fmaxf(fabsf(a.scale_log2), 1e-30f);  // not 0: masked scores are -inf
@@ -773,55 +768,73 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Each sequence's own keys, then the sum with the prefix.  grid (B, KV heads x row chunks, page splits), the splits of
 // a row one cluster.
 template <int D, int NT>
-__global__ void __launch_bounds__(kWarps * 32, kCtas<D, NT>) suffix_kernel(const Args a, int row_chunks) {
-  extern __shared__ __align__(16) uint8_t smem[];
+__global__ void __launch_bounds__(kMaxWarps * 32) 
+    suffix_kernel(const __grid_constant__ CUtensorMap tm, const Args a, int row_chunks) {
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  __shared__ int abort_flag;
+  if (threadIdx.x == 0) abort_flag = 0;
+  __syncthreads();
   const int b = blockIdx.x, kh = blockIdx.y / row_chunks, r0 = blockIdx.y % row_chunks * (NT * 8);
   const int G = a.nq / a.nkv, rows = min(NT * 8, a.ql * G - r0);
   const int splits = gridDim.z, me = blockIdx.z;
-  const Group gr = a.groups[a.seq_group[b]];
+  const int2 sh = __ldg(a.seqs + b);
   const int len = seq_len(a, b);
   // this CTA's pages of [prefix, len)
-  const int begin = min(gr.prefix, len), p0 = begin / PAGE, pages = (len + PAGE - 1) / PAGE - p0;
+  const int begin = min(sh.x, len), p0 = begin / PAGE, pages = (len + PAGE - 1) / PAGE - p0;
   const int per = (pages + splits - 1) / splits;
   const int k0 = max(begin, (p0 + me * per) * PAGE), k1 = min(len, (p0 + (me + 1) * per) * PAGE);
-  float* res = stream<D, NT>(a, smem, a.table + (long)b * a.table_stride, kh, (long)b * a.ql, r0, rows,
-                             min(k0, max(k1, 0)), k1, [&](int r) { return len - a.ql + (r0 + r) / G; });
+  float* res = stream<D, NT>(tm, a, smem, &abort_flag, a.table + (long)b * a.table_stride, kh, (long)b * a.ql, r0, rows,
+                             min(k0, max(k1, 0)), k1, [&](int r) { return len - a.ql + div_g(a, r0 + r); });
   constexpr int RS = D + 2;
   cg::cluster_group cl = cg::this_cluster();
   if (splits > 1) cl.sync();
   griddep_wait();
-  const int n_prefix = gr.prefix > 0 ? (gr.prefix + gr.chunk - 1) / gr.chunk * a.parts : 0;
-  // one warp per row: the weights of all parts, then the sum; the rows are dealt over the CTAs of the cluster
-  for (int r = me * kWarps + warp_id(); r < rows; r += splits * kWarps) {
+  const int n_prefix = sh.y * a.parts;
+  // one warp per row, part s of the prefix in lane s & 31; the rows are dealt over the CTAs of the cluster
+  const int warps = blockDim.x / 32;
+  for (int r = me * warps + warp_id(); r < rows; r += splits * warps) {
     const int lane = lane_id();
-    const long tok = (long)b * a.ql + (r0 + r) / G;
-    const int h = kh * G + (r0 + r) % G;
+    const int qi = div_g(a, r0 + r);
+    const long tok = (long)b * a.ql + qi;
+    const int h = kh * G + (r0 + r - qi * G);
     const long at0 = tok * a.nq + h, step = (long)a.B * a.ql * a.nq;
-    float M = kNegBig;
-    for (int s = 0; s < splits; ++s) M = fmaxf(M, (splits > 1 ? cl.map_shared_rank(res, s) : res)[r * RS + D]);
-    for (int s = lane; s < n_prefix; s += 32) M = fmaxf(M, a.part_ml[at0 + s * step].x);
-    M = warp_max(M);
-    float L = 0.f, O[D / 32];
+    float M = kNegBig, L = 0.f, O[D / 32];
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) O[c] = 0.f;
+    // adds a part (m, l, O / this lane's dims) to the running sum
+    auto scale_to = [&](float m) {
+      const float m_new = fmaxf(M, m), f = exp2f(M - m_new);
+      M = m_new;
+      L *= f;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) O[c] *= f;
+    };
     for (int s = 0; s < splits; ++s) {
       const float* p = (splits > 1 ? cl.map_shared_rank(res, s) : res) + r * RS;
+      scale_to(p[D]);
       const float w = exp2f(p[D] - M);
       L += p[D + 1] * w;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) O[c] += p[lane * (D / 32) + c] * w;
     }
-    for (int s = 0; s < n_prefix; ++s) {
-      const float2 ml = a.part_ml[at0 + s * step];
+    for (int s0 = 0; s0 < n_prefix; s0 += 32) {
+      const int n = min(32, n_prefix - s0);
+      const float2 ml = lane < n ? a.part_ml[at0 + (s0 + lane) * step] : make_float2(kNegBig, 0.f);
+      scale_to(warp_max(ml.x));
       const float w = exp2f(ml.x - M);
-      L += ml.y * w;
-      const float* p = a.part_o + (at0 + s * step) * D + lane * (D / 32);
-      if constexpr (D == 128) {
-        const float4 v = *reinterpret_cast<const float4*>(p);
-        O[0] += v.x * w, O[1] += v.y * w, O[2] += v.z * w, O[3] += v.w * w;
-      } else {
-        const float2 v = *reinterpret_cast<const float2*>(p);
-        O[0] += v.x * w, O[1] += v.y * w;
+      L += warp_sum(ml.y * w);
+      const float* p = a.part_o + (at0 + s0 * step) * D + lane * (D / 32);
+#pragma unroll 4
+      for (int s = 0; s < n; ++s, p += step * D) {
+        const float ws = __shfl_sync(0xffffffffu, w, s);
+        if constexpr (D == 128) {
+          const float4 v = *reinterpret_cast<const float4*>(p);
+          O[0] += v.x * ws, O[1] += v.y * ws, O[2] += v.z * ws, O[3] += v.w * ws;
+        } else {
+          const float2 v = *reinterpret_cast<const float2*>(p);
+          O[0] += v.x * ws, O[1] += v.y * ws;
+        }
       }
     }
     const float inv = L > 0.f ? 1.f / L : 0.f;  // a row that sees nothing gives zeros
@@ -836,11 +849,12 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, NT>) suffix_kernel(const
 }
 
 template <int D, int NT>
-void launch_prefix(const Args& a, int items, cudaStream_t stream) {
-  constexpr int smem = stream_smem<D, NT>(NT * 8);
+void launch_prefix(const CUtensorMap& tm, const Args& a, int items, cudaStream_t stream) {
+  constexpr int kWarps = 4;
+  const int smem = stream_smem<D>(kWarps, NT * 8);
   C10_CUDA_CHECK(
       cudaFuncSetAttribute(prefix_stream_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  prefix_stream_kernel<D, NT><<<dim3(items, a.nkv), kWarps * 32, smem, stream>>>(a);
+  prefix_stream_kernel<D, NT><<<dim3(items, a.nkv), kWarps * 32, smem, stream>>>(tm, a);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
@@ -854,14 +868,20 @@ void launch_prefix_tc(const CUtensorMap& tm, const Args& a, int items, cudaStrea
 }
 
 template <int D, int NT>
-void launch_suffix(const Args& a, int splits, bool dependent, cudaStream_t stream) {
-  const int smem = stream_smem<D, NT>(std::min(NT * 8, a.ql * (a.nq / a.nkv)));
-  C10_CUDA_CHECK(cudaFuncSetAttribute(suffix_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      stream_smem<D, NT>(NT * 8)));
+void launch_suffix(const CUtensorMap& tm, const Args& a, int splits, bool dependent, int sms, cudaStream_t stream) {
   const int row_chunks = (a.ql * (a.nq / a.nkv) + NT * 8 - 1) / (NT * 8);
+  // Warps per sequence, KV head and row chunk: as many as fill the SMs once.  Each warp costs its start and its share
+  // of the merge, so where there are sequences enough one warp takes a whole one: 256 sequences x 8 heads of 1 to 511
+  // tokens took 79 us with four warps each, XX us with one.
+  const long ctas = (long)a.B * a.nkv * row_chunks * splits;
+  int warps = 1;
+  while (warps * 2 <= kMaxWarps && ctas * warps * 2 <= (long)sms * kMaxWarps) warps *= 2;
+  const int smem = stream_smem<D>(warps, std::min(NT * 8, a.ql * (a.nq / a.nkv)));
+  C10_CUDA_CHECK(cudaFuncSetAttribute(suffix_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      stream_smem<D>(kMaxWarps, NT * 8)));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.B, a.nkv * row_chunks, splits);
-  cfg.blockDim = dim3(kWarps * 32);
+  cfg.blockDim = dim3(warps * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute at[2];
@@ -877,22 +897,23 @@ void launch_suffix(const Args& a, int splits, bool dependent, cudaStream_t strea
   }
   cfg.attrs = at;
   cfg.numAttrs = n;
-  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, suffix_kernel<D, NT>, a, row_chunks));
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, suffix_kernel<D, NT>, tm, a, row_chunks));
 }
 
 template <int D>
-void run(const CUtensorMap& tm, const Args& a, int items, int tile_rows, int suffix_splits, cudaStream_t stream) {
+void run(const CUtensorMap& tm, const Args& a, int items, int tile_rows, int suffix_splits, int sms,
+         cudaStream_t stream) {
   if (items > 0) {
-    if (tile_rows == 8) launch_prefix<D, 1>(a, items, stream);
-    else if (tile_rows == 16) launch_prefix<D, 2>(a, items, stream);
-    else if (tile_rows == 32) launch_prefix<D, 4>(a, items, stream);
+    if (tile_rows == 8) launch_prefix<D, 1>(tm, a, items, stream);
+    else if (tile_rows == 16) launch_prefix<D, 2>(tm, a, items, stream);
+    else if (tile_rows == 32) launch_prefix<D, 4>(tm, a, items, stream);
     else if (tile_rows == 128) launch_prefix_tc<D, false>(tm, a, items, stream);
     else launch_prefix_tc<D, true>(tm, a, items, stream);
   }
   const int rows = a.ql * (a.nq / a.nkv);
-  if (rows <= 8) launch_suffix<D, 1>(a, suffix_splits, items > 0, stream);
-  else if (rows <= 16) launch_suffix<D, 2>(a, suffix_splits, items > 0, stream);
-  else launch_suffix<D, 4>(a, suffix_splits, items > 0, stream);
+  if (rows <= 8) launch_suffix<D, 1>(tm, a, suffix_splits, items > 0, sms, stream);
+  else if (rows <= 16) launch_suffix<D, 2>(tm, a, suffix_splits, items > 0, sms, stream);
+  else launch_suffix<D, 4>(tm, a, suffix_splits, items > 0, sms, stream);
 }
 
 }  // namespace shared_prefix
@@ -903,7 +924,7 @@ void run(const CUtensorMap& tm, const Args& a, int items, int tile_rows, int suf
 
 void shared_prefix_attention(const torch::Tensor& q, const torch::Tensor& kv_cache, int64_t layer,
                              const torch::Tensor& block_table, const torch::Tensor& seq_lens, torch::Tensor& out,
-                             const torch::Tensor& items, const torch::Tensor& groups, const torch::Tensor& seq_group,
+                             const torch::Tensor& items, const torch::Tensor& groups, const torch::Tensor& seqs,
                              int64_t q_len, int64_t tile_rows, int64_t prefix_splits, int64_t suffix_splits,
                              double scale) {
   using namespace shared_prefix;
@@ -927,7 +948,8 @@ void shared_prefix_attention(const torch::Tensor& q, const torch::Tensor& kv_cac
                   (block_table.size(1) <= 1 || block_table.stride(1) == 1),
               "block_table must be int32 [B, W] with contiguous rows");
   SP_CHECK(q_len >= 1 && q.size(0) == B * q_len, "q must have batch x q_len rows");
-  SP_CHECK(seq_group.scalar_type() == at::kInt && seq_group.is_contiguous() && seq_group.numel() == B, "the plan is for another number of sequences");
+  SP_CHECK(seqs.scalar_type() == at::kInt && seqs.dim() == 2 && seqs.size(1) == 2 && seqs.is_contiguous() &&
+               seqs.size(0) == B, "the plan is for another number of sequences");
   SP_CHECK(items.scalar_type() == at::kInt && items.dim() == 2 && items.size(1) == 4 && items.is_contiguous() &&
                   groups.scalar_type() == at::kInt && groups.dim() == 2 && groups.size(1) == 4 &&
                   groups.is_contiguous(),
@@ -939,7 +961,7 @@ void shared_prefix_attention(const torch::Tensor& q, const torch::Tensor& kv_cac
   SP_CHECK(nkv * q.size(1) * q_len <= 65535, "too many heads");
   SP_CHECK(q.is_cuda(), "tensors must be on a CUDA device");
   for (const torch::Tensor* t : {&kv_cache, &block_table, &seq_lens, &static_cast<const torch::Tensor&>(out), &items,
-                                 &groups, &seq_group})
+                                 &groups, &seqs})
     SP_CHECK(t->device() == q.device(), "tensors must be on one device");
   if (B == 0) return;
   const at::cuda::CUDAGuard guard(q.device());
@@ -956,11 +978,14 @@ void shared_prefix_attention(const torch::Tensor& q, const torch::Tensor& kv_cac
   a.lens = seq_lens.data_ptr<int>();
   a.items = reinterpret_cast<const int4*>(items.data_ptr<int>());
   a.groups = reinterpret_cast<const Group*>(groups.data_ptr<int>());
-  a.seq_group = seq_group.data_ptr<int>();
+  a.seqs = reinterpret_cast<const int2*>(seqs.data_ptr<int>());
   a.B = int(B);
   a.nq = int(nq);
   a.nkv = int(nkv);
   a.ql = int(q_len);
+  const int64_t G = nq / nkv;
+  SP_CHECK(T * G * G < (1ll << 32), "too many query rows");
+  a.per_g = G > 1 ? uint32_t(((1ull << 32) + G - 1) / G) : 0;
   a.NB = int(kv_cache.size(1));
   a.scale_log2 = float(scale * 1.4426950408889634);
   a.status = status_word(q.get_device());
@@ -971,10 +996,10 @@ void shared_prefix_attention(const torch::Tensor& q, const torch::Tensor& kv_cac
   a.part_o = ws.data_ptr<float>();
   a.part_ml = reinterpret_cast<float2*>(a.part_o + prefix_splits * T * nq * D);
   const auto* base = reinterpret_cast<const __nv_bfloat16*>(kv_cache.data_ptr()) + layer * kv_cache.stride(0);
-  a.kv = base;
   const CUtensorMap tm = make_tmap_bf16_2d(base, D, rows, D * 2, 64, PAGE);
-  if (D == 128) run<128>(tm, a, int(items.size(0)), int(tile_rows), int(suffix_splits), stream);
-  else run<64>(tm, a, int(items.size(0)), int(tile_rows), int(suffix_splits), stream);
+  const int sms = num_sms(q.get_device());
+  if (D == 128) run<128>(tm, a, int(items.size(0)), int(tile_rows), int(suffix_splits), sms, stream);
+  else run<64>(tm, a, int(items.size(0)), int(tile_rows), int(suffix_splits), sms, stream);
 }
 
 }  // namespace bloom

@@ -17,7 +17,7 @@ def i32(*v):
 def test_plan_covers_every_row_and_key_once(sizes, prefix, heads):
     nq, nkv, D, ql = heads
     p = ops.shared_prefix_plan(sizes, prefix, num_q_heads=nq, num_kv_heads=nkv, head_dim=D, q_len=ql)
-    assert p.batch == sum(sizes) and p.seq_group.tolist() == [g for g, n in enumerate(sizes) for _ in range(n)]
+    assert p.batch == sum(sizes)
     seen = {}
     for g, r0, s, _ in p.items.tolist():
         first, members, pre, chunk = p.groups[g].tolist()
@@ -25,6 +25,8 @@ def test_plan_covers_every_row_and_key_once(sizes, prefix, heads):
         assert s < p.prefix_splits and s * chunk < pre and r0 % p.tile_rows == 0 and r0 < members * ql * (nq // nkv)
         assert (g, r0, s) not in seen
         seen[g, r0, s] = min(chunk, pre - s * chunk)
+    splits = [max([s + 1 for (gg, _, s) in seen if gg == g], default=0) for g in range(len(sizes))]
+    assert p.seqs.tolist() == [[prefix[g], splits[g]] for g, n in enumerate(sizes) for _ in range(n)]
     for g, (n, pre) in enumerate(zip(sizes, prefix)):
         rows = n * ql * (nq // nkv)
         for r0 in range(0, rows, p.tile_rows):
