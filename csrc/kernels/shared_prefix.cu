@@ -110,9 +110,11 @@ __device__ __forceinline__ int block_id(const Args& a, const int* row, int page)
 // The member of a group whose table row the prefix is read through: the first that holds the most of it (members that
 // have ended, of length 0, are passed over).  Every lane of the calling warp gets {member, prefix tokens it holds}.
 __device__ __forceinline__ int2 prefix_holder(const Args& a, const Group& g) {
+  // lengths are taken into the table row; the suffix kernel reports those that are not in it
   unsigned long long best = 0;
+#pragma unroll 8
   for (int i = lane_id(); i < g.members; i += 32) {
-    const int n = min(seq_len(a, g.first + i), g.prefix);
+    const int n = max(0, min(min(__ldg(a.lens + g.first + i), a.W * PAGE), g.prefix));
     const unsigned long long v = (static_cast<unsigned long long>(n) << 32) | (0xffffffffu - unsigned(i));
     best = v > best ? v : best;
   }
@@ -427,6 +429,30 @@ __device__ __forceinline__ void pin(float (&v)[16]) {
                : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
                  "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]));
 }
+// Two fp32 operations in one instruction, and the largest of three.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 // D[tmem] (+)= A[tmem] B[smem desc], A: lane = row, two consecutive bf16 k per 32-bit column
 __device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t acc) {
   asm volatile(
@@ -632,10 +658,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (kPair || w == 0) {  // this thread's q row, K-major with the 128-byte swizzle
       const uint4* src = reinterpret_cast<const uint4*>(a.q + token * a.q_stride + (long)h * D);
       uint8_t* dst = sQ + (kPair ? w * C::kQ : 0) + t * 128;
+      uint4 x[D / 8];  // all of it requested before the first store
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) x[c] = __ldg(src + c);
 #pragma unroll
       for (int c = 0; c < D / 8; ++c)
         *reinterpret_cast<uint4*>(dst + (c >> 3) * (kRows * 128) + (((c & 7) ^ (t & 7)) << 4)) =
-            valid ? flip(src[c]) : make_uint4(0, 0, 0, 0);
+            valid ? flip(x[c]) : make_uint4(0, 0, 0, 0);
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_ready);
@@ -669,11 +698,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int e = 0; e < 16; ++e) v[c][e] = kv0 + 16 * c + e <= limit ? v[c][e] : -INFINITY;
         }
-        float mx = -INFINITY;
+        float mc[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 4; ++c) {
+          mc[c] = fmaxf(v[c][0], v[c][1]);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) mx = fmaxf(mx, v[c][e]);
+          for (int e = 2; e < 16; e += 2) mc[c] = max3(mc[c], v[c][e], v[c][e + 1]);
+        }
+        const float mx = fmaxf(max3(mc[0], mc[1], mc[2]), mc[3]);
         const float m_new = fmaxf(m, mx == -INFINITY ? kNegBig : mx * scale);
         const bool grow = m_new > m + kLazy || i == 0;
         const float alpha = grow ? exp2f(m - m_new) : 1.f;
@@ -699,20 +731,34 @@ __global__ void __launch_bounds__(kThreads, 1)
           l *= alpha;
           m = m_new;
         }
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t sc2 = pack2(scale, scale), m2 = pack2(-m, -m);
+        uint64_t sum[4] = {0, 0, 0, 0};
+        // in steps over the whole tile, so that every step has 32 or 64 independent operations
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {  // 32 keys -> 16 columns of P
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) unpack2(fma2(pack2(v[c][e], v[c][e + 1]), sc2, m2), v[c][e], v[c][e + 1]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) v[c][e] = exp2f(v[c][e]);
+          pin(v[c]);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; c += 2) {  // 32 keys -> 16 columns of P
           uint32_t u[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float p0 = exp2f(fmaf(v[2 * c + (e >> 3)][(2 * e) & 15], scale, -m));
-            const float p1 = exp2f(fmaf(v[2 * c + (e >> 3)][(2 * e + 1) & 15], scale, -m));
-            sum[e & 3] += p0 + p1;
-            u[e] = pack_bf16x2(p0, p1);  // rounded by 2^-8 at most; l keeps the fp32 sum
-          }
-          tmem_st_x16(tS + 16 * c, u);
+          for (int e = 0; e < 16; ++e)  // rounded by 2^-8 at most; l keeps the fp32 sum
+            u[e] = pack_bf16x2(v[c + (e >> 3)][2 * (e & 7)], v[c + (e >> 3)][2 * (e & 7) + 1]);
+          tmem_st_x16(tS + 8 * c, u);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) sum[c] = add2(sum[c], pack2(v[c][e], v[c][e + 1]));
+        float s0, s1;
+        unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), s0, s1);
+        l += s0 + s1;
         tmem_wait_st();
       }
       if (kv0 + kKv > k1) {  // V rows behind the last key: whatever they hold must not meet p = 0
