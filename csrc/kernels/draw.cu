@@ -3,26 +3,31 @@
 //   w_i = exp((l_i - max) / t)                        (l = NaN counts as -inf)
 //   top-k  keeps the k largest, ties to the lowest index
 //   top-p  keeps, in falling order, every token with less than p Z ahead of it (Z: the mass that top-k keeps)
-//   min-p  keeps w_i >= min_p
+//   min-p  keeps w_i >= min_p, i.e. l_i >= max + t ln(min_p)
 //   token  the first kept i in vocabulary order whose inclusive sum exceeds u Z_kept
 //
-// The token is a whole number, so sums decide it at borders: weights are computed in fp64 (error ~1e-16) and summed as
-// 64-bit fixed point with 2^45 for the largest.  Integer sums are exact and do not depend on the order of atomics, so
-// a call gives the same tokens every time.  Weights below 2^-46 of the largest count as zero.
+// The token is a whole number, so sums decide it at borders: weights are computed in fp64 (error below 1e-11) and summed
+// as 64-bit fixed point with 2^45 for the largest.  Integer sums are exact and do not depend on the order of atomics,
+// so a call gives the same tokens every time.  Weights below 2^-46 of the largest (32 t below the maximum) count as 0.
 //
 // One cluster of C CTAs per row, each CTA holding a slice of the row in shared memory, so a row is read from HBM once
-// however many passes follow.  The cut of top-k / top-p is found by histograms of 1024 bins: first over the scaled
-// distance to the maximum, (max - l) / t in 30 / 1023 steps, which spreads real logits over many bins where their
-// floating-point bits would crowd a few; then over the bits of the values inside the bin that holds the cut, until it
-// is one value.  Each histogram is reduced over the cluster through distributed shared memory (each CTA sums its
-// share of the bins and stores the sums into all CTAs).  Mass sums use two 32-bit shared atomics with a carry.
-// The draw walks vocabulary order: sums of 256-token chunks, a scan, and one warp for the chunk that holds u Z.
+// however many passes follow.  The passes are bound by instructions (a weight takes about 20), so the cut of top-k / top-p
+// avoids weights where it can:
+//   1. counts in 1024 bins over the distance to the maximum, (max - l) / t in steps of 1 / 32
+//   2. top-k: the bin that holds the k-th is gathered into one CTA, sorted by (value, index), and cut
+//   3. top-p: counts bound the mass of a bin to 3%, which leaves a window of bins for the cut; one pass sums the exact
+//      masses before, behind, and per bin of the window; the bin that holds the cut is gathered, sorted and cut
+// A bin of more than kList tokens (many equal values) is instead narrowed by histograms over the bits of its values,
+// and equal values are counted off in vocabulary order.  Histograms are reduced over the cluster through distributed
+// shared memory.  The draw walks vocabulary order: sums of 256 tokens, a scan, and one warp for the chunk that
+// holds u Z.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cooperative_groups.h>
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <cfloat>
 
 #include "bloom/common.cuh"
 #include "bloom/ops_share.h"
@@ -40,8 +45,10 @@ constexpr int kChunk = 256;          // tokens of one warp step: 8 consecutive o
 constexpr int kMaxCluster = 8;
 constexpr int64_t kMaxVocab = 1 << 18;  // sums of 2^45 stay below 2^63
 constexpr int kMaxSliceBytes = 128 * 1024;
-constexpr float kRange = 30.f;
-constexpr int kTab = 64;
+constexpr float kRange = 32.f;       // in units of t below the maximum; e^-32 < 2^-46
+constexpr float kBinsPerT = kBins / kRange;
+constexpr int kTab = 1024;
+constexpr int kList = 2048;          // tokens that one CTA sorts
 
 using u64 = unsigned long long;
 
@@ -60,128 +67,136 @@ struct Args {
   bool vec;              // rows start on 16-byte boundaries
 };
 
+struct Hist {
+  unsigned cnt[kBins], lo[kBins], hi[kBins];  // this CTA's counts and masses
+};
+// What top-k / top-p keep: values above `v`, and of those equal to it the ones at or before `last`.
+struct Cut {
+  float v;
+  int last;
+};
 struct Shared {
-  double tab[kTab];                    // 2^(j / 64)
-  unsigned cnt[kBins], lo[kBins], hi[kBins];  // this CTA's histogram
-  u64 mass[2][kBins];                  // the cluster's, scanned: [0] first level, [1] the finer ones
-  unsigned count[2][kBins];
+  double tab[kTab];                    // 2^45 2^(j / 1024)
+  union {
+    Hist h;
+    u64 list[kList];                   // (order-preserving bits of the value, ~index)
+  };
+  unsigned count[2][kBins];            // the cluster's counts, scanned: [0] first level, [1] the finer ones
+  u64 mass[kBins];
   u64 wsum[kWarps];
+  double wlo[kWarps], whi[kWarps];
   unsigned wcnt[kWarps];
   float cl_max[kMaxCluster];           // written by the CTAs of the cluster
   int cl_arg[kMaxCluster];
   unsigned cl_lo[2][kMaxCluster], cl_hi[2][kMaxCluster];  // one for each of a row's two selections
   unsigned cl_cnt[kMaxCluster];
-  u64 cl_mass[kMaxCluster];
+  u64 cl_above[kMaxCluster], cl_all[kMaxCluster], cl_mass[kMaxCluster];
+  Cut cl_cut[2];
   int cl_index;
-  unsigned found;
+  unsigned n_list;
+  unsigned found, found2;
   float red_f[kWarps];
-  int red_i[kWarps];
   unsigned red_a[kWarps], red_b[kWarps];
 };
 
-template <typename T>
-__device__ __forceinline__ float clean(T v);
-// NaN -> -inf, -0 -> +0
-template <>
-__device__ __forceinline__ float clean<float>(float v) {
-  return v == v ? v + 0.f : -INFINITY;
-}
-template <>
-__device__ __forceinline__ float clean<__nv_bfloat16>(__nv_bfloat16 v) {
-  return clean<float>(__bfloat162float(v));
-}
-// Order-preserving bits of a float.
+// Order-preserving bits of a float (-0 as +0).
 __device__ __forceinline__ unsigned key_of(float v) {
-  const unsigned b = __float_as_uint(v);
+  const unsigned b = __float_as_uint(v + 0.f);
   return b ^ (static_cast<unsigned>(static_cast<int>(b) >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float value_of(unsigned key) {
   return __uint_as_float(key ^ ((key & 0x80000000u) ? 0x80000000u : 0xffffffffu));
 }
 
-// exp(x) for x in (-32, 0] as 2^k 2^(j/64) e^r with |r| <= ln 2 / 128: a table of powers and the Taylor polynomial
-// of degree 5 (remainder r^6 / 720 < 4e-17).  The rounding to n = 64 k + j adds 1.5 2^52, whose low bits are n.
-__device__ __forceinline__ double exp_neg(double x, const double* tab) {
-  constexpr double kMagic = 6755399441055744.0;
-  const double z = fma(x, 92.332482616893656877, kMagic);  // 64 / ln 2
-  const int n = __double2loint(z);
-  const double r = fma(z - kMagic, -0.010830424696249145, x);  // ln 2 / 64
-  double p = fma(r, 1.0 / 120, 1.0 / 24);
-  p = fma(r, p, 1.0 / 6);
-  p = fma(r, p, 0.5);
-  p = fma(r, p, 1.0);
-  p = fma(r, p, 1.0);
-  const double v = tab[n & (kTab - 1)] * p;
-  return __hiloint2double(__double2hiint(v) + ((n >> 6) << 20), __double2loint(v));
-}
-
 struct Row {
-  float mx, inv_tf;
-  double mxd, inv_t, min_w;
+  float mx, bins;      // bins per unit of l
+  float low;           // values below it have no mass
+  double mxd, c;       // the maximum, 1024 / (t ln 2)
 };
-__device__ __forceinline__ double weight(float l, const Row& r, const double* tab) {
-  if (l == r.mx) return 1.0;
-  if (!(l > -INFINITY)) return 0.0;
-  const double x = (static_cast<double>(l) - r.mxd) * r.inv_t;
-  return x > -32.0 ? exp_neg(x, tab) : 0.0;
+// round(2^45 exp((l - max) / t)) for l >= low: y = 1024 (l - max) / (t ln 2) = n + f with n = 1024 k + j, then
+// 2^k 2^(j / 1024) e^(f ln 2 / 1024): a table of powers, and 1 + x + x^2 / 2 for |x| < 3.4e-4 (remainder < 7e-12).  The
+// rounding to n adds 1.5 2^52, whose low bits are n; the rounding to a whole mass adds 2^52.
+__device__ __forceinline__ u64 mass_of(float l, const Row& r, const double* tab) {
+  constexpr double kMagic = 6755399441055744.0, a = 6.7690154351557157e-4;  // ln 2 / 1024
+  const double y = (static_cast<double>(l) - r.mxd) * r.c;  // the difference is exact, or nearly: logits may be large
+  const double z = y + kMagic;
+  const int n = __double2loint(z);
+  const double f = y - (z - kMagic);
+  const double p = fma(f, fma(f, 0.5 * a * a, a), 1.0);
+  const double v = tab[n & (kTab - 1)] * p;
+  const double w = __hiloint2double(__double2hiint(v) + ((n & ~(kTab - 1)) << 10), __double2loint(v));
+  return static_cast<u64>(__double_as_longlong(w + 4503599627370496.0)) & 0xfffffffffffffull;
 }
-// round(w 2^45): the low 52 bits of w 2^45 + 2^52
-__device__ __forceinline__ u64 fixed(double w) {
-  return static_cast<u64>(__double_as_longlong(fma(w, 35184372088832.0, 4503599627370496.0))) & 0xfffffffffffffull;
+// What a cut keeps, for all values including those below low, and the mass then.  Without a branch: in one, a warp
+// runs the 20 instructions of a mass for every token all the same, and as many again to enter and leave it.
+__device__ __forceinline__ bool keeps(const Cut& c, float v, int i) { return v > c.v || (v == c.v && i <= c.last); }
+__device__ __forceinline__ u64 mass_if(bool keep, float v, const Row& r, const double* tab) {
+  const u64 m = mass_of(v, r, tab);
+  return keep ? m : 0;
 }
-__device__ __forceinline__ u64 mass_of(float l, const Row& r, const double* tab) { return fixed(weight(l, r, tab)); }
-// First-level bin: monotone in l, because every rounding in it is.
+// First-level bin of l >= low: monotone in l, because every rounding in it is.
 __device__ __forceinline__ int bin_of(float l, const Row& r) {
-  if (l == r.mx) return 0;
-  const float x = (r.mx - l) * r.inv_tf;
-  return x < kRange ? static_cast<int>(x * ((kBins - 1) / kRange)) : kBins - 1;
+  return min(static_cast<int>((r.mx - l) * r.bins), kBins - 1);
 }
 
-// f(chunk, first index within the slice, 8 values) for this warp's chunks.
+// 8 consecutive tokens from the slice.
+template <typename T>
+__device__ __forceinline__ void load8(const T* at, float (&v)[8]) {
+  const uint4* p = reinterpret_cast<const uint4*>(at);
+  if constexpr (sizeof(T) == 2) {
+    const uint4 a = p[0];
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  } else {
+    const uint4 a = p[0], b = p[1];
+    v[0] = __uint_as_float(a.x), v[1] = __uint_as_float(a.y), v[2] = __uint_as_float(a.z);
+    v[3] = __uint_as_float(a.w), v[4] = __uint_as_float(b.x), v[5] = __uint_as_float(b.y);
+    v[6] = __uint_as_float(b.z), v[7] = __uint_as_float(b.w);
+  }
+}
+// f(first index within the slice, 8 values) for this warp's chunks.
 template <typename T, typename F>
 __device__ __forceinline__ void for_chunks(const T* sl, int chunks, F&& f) {
   const int lane = lane_id();
   for (int c = warp_id(); c < chunks; c += kWarps) {
     float v[8];
-    const uint4* p = reinterpret_cast<const uint4*>(sl + c * kChunk + lane * 8);
-    if constexpr (sizeof(T) == 2) {
-      const uint4 a = p[0];
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      }
-    } else {
-      const uint4 a = p[0], b = p[1];
-      v[0] = __uint_as_float(a.x), v[1] = __uint_as_float(a.y), v[2] = __uint_as_float(a.z);
-      v[3] = __uint_as_float(a.w), v[4] = __uint_as_float(b.x), v[5] = __uint_as_float(b.y);
-      v[6] = __uint_as_float(b.z), v[7] = __uint_as_float(b.w);
-    }
-    f(c, c * kChunk + lane * 8, v);
+    load8(sl + c * kChunk + lane * 8, v);
+    f(c * kChunk + lane * 8, v);
   }
 }
+__device__ __forceinline__ u64 warp_sum_u64(u64 m) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
+  return m;
+}
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 
 template <typename P>
 __device__ __forceinline__ P* remote(cg::cluster_group& cl, P* p, int rank) {
   return cl.map_shared_rank(p, rank);
 }
 
-__device__ __forceinline__ void clear_hist(Shared& s) {
-  for (int b = threadIdx.x; b < kBins; b += kThreads) s.cnt[b] = s.lo[b] = s.hi[b] = 0;
-}
-__device__ __forceinline__ void hist_add(Shared& s, int b, bool with_mass, u64 m) {
-  atomicAdd(&s.cnt[b], 1u);
-  if (with_mass) {
-    const unsigned l = static_cast<unsigned>(m);
-    const unsigned before = atomicAdd(&s.lo[b], l);
-    const unsigned up = static_cast<unsigned>(m >> 32) + (before + l < before ? 1u : 0u);
-    if (up) atomicAdd(&s.hi[b], up);
+__device__ __forceinline__ void clear_hist(Shared& s, bool with_mass) {
+  for (int b = threadIdx.x; b < kBins; b += kThreads) {
+    s.h.cnt[b] = 0;
+    if (with_mass) s.h.lo[b] = s.h.hi[b] = 0;
   }
 }
+// 64-bit sums as two 32-bit atomics and a carry: integer adds of 64 bits are not native to shared memory
+__device__ __forceinline__ void hist_mass(Shared& s, int b, u64 m) {
+  const unsigned l = static_cast<unsigned>(m);
+  const unsigned before = atomicAdd(&s.h.lo[b], l);
+  const unsigned up = static_cast<unsigned>(m >> 32) + (before + l < before ? 1u : 0u);
+  if (up) atomicAdd(&s.h.hi[b], up);
+}
 
-// The cluster's histogram, inclusively scanned, into count[lv] / mass[lv] of every CTA.
-__device__ void combine(cg::cluster_group& cl, Shared& s, int lv) {
+// The cluster's histogram, inclusively scanned, into count[lv] (counts) / mass (masses) of every CTA.
+__device__ void combine(cg::cluster_group& cl, Shared& s, int lv, bool counts, bool masses) {
   const int C = cl.num_blocks(), me = cl.block_rank();
   cl.sync();
   const int share = kBins / C;
@@ -191,20 +206,20 @@ __device__ void combine(cg::cluster_group& cl, Shared& s, int lv) {
     u64 m = 0;
     for (int r = 0; r < C; ++r) {
       const Shared* o = remote(cl, &s, r);
-      c += o->cnt[b];
-      m += (static_cast<u64>(o->hi[b]) << 32) + o->lo[b];
+      if (counts) c += o->h.cnt[b];
+      if (masses) m += (static_cast<u64>(o->h.hi[b]) << 32) + o->h.lo[b];
     }
     for (int r = 0; r < C; ++r) {
       Shared* o = remote(cl, &s, r);
-      o->count[lv][b] = c;
-      o->mass[lv][b] = m;
+      if (counts) o->count[lv][b] = c;
+      if (masses) o->mass[b] = m;
     }
   }
   cl.sync();
   // block scan, two bins per thread
   const int lane = lane_id(), w = warp_id(), b0 = 2 * threadIdx.x;
-  const unsigned c0 = s.count[lv][b0], c1 = s.count[lv][b0 + 1];
-  const u64 m0 = s.mass[lv][b0], m1 = s.mass[lv][b0 + 1];
+  const unsigned c0 = counts ? s.count[lv][b0] : 0, c1 = counts ? s.count[lv][b0 + 1] : 0;
+  const u64 m0 = masses ? s.mass[b0] : 0, m1 = masses ? s.mass[b0 + 1] : 0;
   unsigned c = c0 + c1;
   u64 m = m0 + m1;
 #pragma unroll
@@ -219,20 +234,18 @@ __device__ void combine(cg::cluster_group& cl, Shared& s, int lv) {
   u64 mb = 0;
   for (int i = 0; i < w; ++i) cb += s.wcnt[i], mb += s.wsum[i];
   c += cb, m += mb;
-  s.count[lv][b0] = c - c1;
-  s.count[lv][b0 + 1] = c;
-  s.mass[lv][b0] = m - m1;
-  s.mass[lv][b0 + 1] = m;
+  if (counts) s.count[lv][b0] = c - c1, s.count[lv][b0 + 1] = c;
+  if (masses) s.mass[b0] = m - m1, s.mass[b0 + 1] = m;
   __syncthreads();
 }
 
-// First bin whose inclusive count or mass reaches `target`.
-__device__ int find(Shared& s, int lv, bool by_mass, u64 target) {
+// First bin whose inclusive count (lv) or mass (lv < 0) reaches `target`.
+__device__ int find(Shared& s, int lv, u64 target) {
   if (threadIdx.x == 0) s.found = kBins - 1;
   __syncthreads();
   for (int b = threadIdx.x; b < kBins; b += kThreads) {
-    const u64 v = by_mass ? s.mass[lv][b] : s.count[lv][b];
-    const u64 p = b == 0 ? 0 : by_mass ? s.mass[lv][b - 1] : s.count[lv][b - 1];
+    const u64 v = lv < 0 ? s.mass[b] : s.count[lv][b];
+    const u64 p = b == 0 ? 0 : lv < 0 ? s.mass[b - 1] : s.count[lv][b - 1];
     if (v >= target && p < target) s.found = b;  // at most one bin
   }
   __syncthreads();
@@ -241,27 +254,97 @@ __device__ int find(Shared& s, int lv, bool by_mass, u64 target) {
   return r;
 }
 
-// What top-k / top-p keep: keys above `key`, and of those equal to it the ones at or before `last`.
-struct Cut {
-  unsigned key;
-  int last;
-  u64 mass;  // of all that is kept (only with masses)
-};
-
+// The members of first-level bin `bin` that `cut` keeps (there are `inside` <= kList of them), gathered into CTA 0 and
+// sorted there by falling value, then index.  The cut moves to the first of them whose inclusive count, or mass after
+// `mbefore`, reaches the target.
 template <typename T>
-__device__ Cut select(cg::cluster_group& cl, Shared& s, const T* sl, int chunks, int s0, const Row& row, int sel,
-                      bool by_mass, bool with_mass, u64 target) {
-  const int C = cl.num_blocks(), me = cl.block_rank();
-  const int lane = lane_id(), w = warp_id();
-  int b = find(s, 0, by_mass, target);
-  unsigned before = b ? s.count[0][b - 1] : 0, inside = s.count[0][b] - before;
-  u64 mbefore = b ? s.mass[0][b - 1] : 0, minside = s.mass[0][b] - mbefore;
-  // the smallest and largest key in the bin
-  unsigned lo = 0xffffffffu, hi = 0;
-  for_chunks(sl, chunks, [&](int, int, const float(&v)[8]) {
+__device__ Cut sort_select(cg::cluster_group& cl, Shared& s, const T* sl, int chunks, int s0, const Row& row, int sel,
+                           Cut cut, int bin, unsigned inside, bool by_mass, u64 before, u64 target) {
+  const int me = cl.block_rank(), lane = lane_id(), w = warp_id();
+  Shared* o = remote(cl, &s, 0);
+  for_chunks(sl, chunks, [&](int i, const float(&v)[8]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (bin_of(v[e], row) == b) {
+      if (v[e] >= row.low && bin_of(v[e], row) == bin && (v[e] > cut.v || (v[e] == cut.v && s0 + i + e <= cut.last))) {
+        const unsigned at = atomicAdd(&o->n_list, 1u);
+        if (at < kList)
+          o->list[at] = (static_cast<u64>(key_of(v[e])) << 32) | static_cast<unsigned>(~(s0 + i + e));
+      }
+  });
+  cl.sync();
+  if (me == 0) {
+    int n = 32;
+    while (n < static_cast<int>(inside)) n *= 2;
+    for (int i = inside + threadIdx.x; i < n; i += kThreads) s.list[i] = 0;
+    __syncthreads();
+    for (int k = 2; k <= n; k *= 2)  // bitonic, falling
+      for (int j = k / 2; j > 0; j /= 2) {
+        for (int i = threadIdx.x; i < n / 2; i += kThreads) {
+          const int a = 2 * i - (i & (j - 1)), b = a + j;
+          const u64 x = s.list[a], y = s.list[b];
+          if ((x < y) == ((a & k) == 0)) s.list[a] = y, s.list[b] = x;
+        }
+        __syncthreads();
+      }
+    int pick = -1;
+    if (!by_mass) {
+      pick = static_cast<int>(target - before) - 1;
+    } else {  // inclusive masses in order: each thread a run of 4
+      const int i0 = threadIdx.x * (kList / kThreads);
+      u64 m[kList / kThreads], sum = 0;
+#pragma unroll
+      for (int q = 0; q < kList / kThreads; ++q) {
+        const int i = i0 + q;
+        m[q] = i < static_cast<int>(inside) ? mass_of(value_of(static_cast<unsigned>(s.list[i] >> 32)), row, s.tab) : 0;
+        sum += m[q];
+      }
+      u64 x = sum;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const u64 y = __shfl_up_sync(0xffffffffu, x, d);
+        if (lane >= d) x += y;
+      }
+      if (lane == 31) s.wsum[w] = x;
+      if (threadIdx.x == 0) s.found2 = inside - 1;
+      __syncthreads();
+      u64 acc = before + x - sum;
+      for (int i = 0; i < w; ++i) acc += s.wsum[i];
+#pragma unroll
+      for (int q = 0; q < kList / kThreads; ++q) {
+        if (acc < target && acc + m[q] >= target) s.found2 = i0 + q;  // at most one
+        acc += m[q];
+      }
+      __syncthreads();
+      pick = static_cast<int>(s.found2);
+    }
+    if (threadIdx.x < cl.num_blocks()) {
+      const u64 x = s.list[pick];
+      remote(cl, &s, threadIdx.x)->cl_cut[sel] =
+          Cut{value_of(static_cast<unsigned>(x >> 32)), static_cast<int>(~static_cast<unsigned>(x))};
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) s.n_list = 0;
+  }
+  cl.sync();
+  return s.cl_cut[sel];
+}
+
+// The same for a bin of more tokens: its range of values is narrowed by histograms of their bits until it is one value
+// (or all of it is kept), and equal values are counted off in vocabulary order.
+template <typename T>
+__device__ Cut narrow_select(cg::cluster_group& cl, Shared& s, const T* sl, int chunks, int s0, const Row& row, int sel,
+                             Cut cut, int bin, unsigned inside, u64 minside, bool by_mass, unsigned before, u64 mbefore,
+                             u64 target) {
+  const int C = cl.num_blocks(), me = cl.block_rank();
+  const int lane = lane_id(), w = warp_id();
+  auto member = [&](float v, int i) {
+    return v >= row.low && bin_of(v, row) == bin && (v > cut.v || (v == cut.v && i <= cut.last));
+  };
+  unsigned lo = 0xffffffffu, hi = 0;
+  for_chunks(sl, chunks, [&](int i, const float(&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (member(v[e], s0 + i + e)) {
         const unsigned k = key_of(v[e]);
         lo = min(lo, k);
         hi = max(hi, k);
@@ -279,46 +362,48 @@ __device__ Cut select(cg::cluster_group& cl, Shared& s, const T* sl, int chunks,
   }
   cl.sync();
   for (int r = 0; r < C; ++r) lo = min(lo, s.cl_lo[sel][r]), hi = max(hi, s.cl_hi[sel][r]);
-  // all that is in the bin is kept: no need to look inside
+  // all that is left in the range is kept: no need to look inside
   auto whole = [&]() { return inside == 1 || (by_mass ? mbefore + minside == target : before + inside == target); };
   while (hi != lo && !whole()) {
     const int shift = max(0, 32 - __clz(hi - lo) - 10);
-    clear_hist(s);
+    clear_hist(s, by_mass);
     __syncthreads();
-    for_chunks(sl, chunks, [&](int, int, const float(&v)[8]) {
+    for_chunks(sl, chunks, [&](int i, const float(&v)[8]) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const unsigned k = key_of(v[e]);
-        if (k >= lo && k <= hi)
-          hist_add(s, (hi - k) >> shift, with_mass, with_mass ? mass_of(v[e], row, s.tab) : 0);
-      }
+      for (int e = 0; e < 8; ++e)
+        if (member(v[e], s0 + i + e)) {
+          const unsigned k = key_of(v[e]);
+          if (k >= lo && k <= hi) {
+            atomicAdd(&s.h.cnt[(hi - k) >> shift], 1u);
+            if (by_mass) hist_mass(s, (hi - k) >> shift, mass_of(v[e], row, s.tab));
+          }
+        }
     });
-    combine(cl, s, 1);
-    b = find(s, 1, by_mass, target - (by_mass ? mbefore : before));
+    combine(cl, s, 1, true, by_mass);
+    const int b = by_mass ? find(s, -1, target - mbefore) : find(s, 1, target - before);
     const unsigned cb = b ? s.count[1][b - 1] : 0;
-    const u64 mb = b ? s.mass[1][b - 1] : 0;
     inside = s.count[1][b] - cb;
-    minside = s.mass[1][b] - mb;
     before += cb;
-    mbefore += mb;
+    if (by_mass) {
+      const u64 mb = b ? s.mass[b - 1] : 0;
+      minside = s.mass[b] - mb;
+      mbefore += mb;
+    }
     const unsigned top = hi - (static_cast<unsigned>(b) << shift);
     lo = max(lo, top - ((1u << shift) - 1u));
     hi = top;
   }
-  Cut cut;
-  cut.key = lo;
-  cut.last = 0x7fffffff;
-  cut.mass = mbefore + minside;
-  if (whole()) return cut;
+  const float v = value_of(lo);
+  const int old = v == cut.v ? cut.last : 0x7fffffff;  // of values equal to the previous cut's, those it kept
+  if (whole()) return Cut{v, old};
   // equal values: the first `r` of them by index
-  const u64 one = with_mass ? mass_of(value_of(lo), row, s.tab) : 0;
+  const u64 one = by_mass ? mass_of(v, row, s.tab) : 0;
   const u64 r = by_mass ? (one ? (target - mbefore + one - 1) / one : 1) : target - before;
-  if (r >= inside) return cut;
-  cut.mass = mbefore + r * one;
+  if (r >= inside) return Cut{v, old};
   unsigned mine = 0;
-  for_chunks(sl, chunks, [&](int, int, const float(&v)[8]) {
+  for_chunks(sl, chunks, [&](int, const float(&x)[8]) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) mine += key_of(v[e]) == lo;
+    for (int e = 0; e < 8; ++e) mine += x[e] == v;
   });
   mine = __reduce_add_sync(0xffffffffu, mine);
   if (lane == 0) s.red_a[w] = mine;
@@ -337,7 +422,7 @@ __device__ Cut select(cg::cluster_group& cl, Shared& s, const T* sl, int chunks,
       unsigned hit = 0;
       const T* p = sl + c * kChunk + lane * 8;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) hit |= (key_of(clean<T>(p[e])) == lo ? 1u : 0u) << e;
+      for (int e = 0; e < 8; ++e) hit |= (to_float(p[e]) == v ? 1u : 0u) << e;
       unsigned n = __popc(hit), incl = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -357,12 +442,11 @@ __device__ Cut select(cg::cluster_group& cl, Shared& s, const T* sl, int chunks,
     }
   }
   cl.sync();
-  cut.last = s.cl_index;
-  return cut;
+  return Cut{v, s.cl_index};
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) draw_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, 2) draw_kernel(const Args a) {
   extern __shared__ __align__(16) uint8_t raw[];
   cg::cluster_group cl = cg::this_cluster();
   const int C = cl.num_blocks(), me = cl.block_rank();
@@ -375,103 +459,234 @@ __global__ void __launch_bounds__(kThreads) draw_kernel(const Args a) {
   const int n = max(0, min(a.slice, a.V - s0));
   const int chunks = (n + kChunk - 1) / kChunk;
   const T* row = static_cast<const T*>(a.logits) + (long)b * a.ld + s0;
+  const float t = a.temp[b];
+  const int k = a.top_k != nullptr ? a.top_k[b] : 0;
+  const float p = a.top_p != nullptr ? a.top_p[b] : 1.f;
+  const float mp = a.min_p != nullptr ? a.min_p[b] : 0.f;
 
-  // ---- the slice into shared memory (NaN and the padding as -inf), its maximum
-  if (threadIdx.x < kTab) s.tab[threadIdx.x] = exp2(threadIdx.x / double(kTab));
-  float best = -INFINITY;
-  int arg = 0x7fffffff;
-  auto take = [&](int i, T raw_v) {
-    const float v = clean<T>(raw_v);
-    if (v > best) best = v, arg = s0 + i;  // a thread sees rising indexes: the first of equal ones stays
-    return static_cast<T>(v);
-  };
+  // ---- the slice into shared memory (padding: -inf), its maximum (NaN is never the larger one)
   constexpr int kVec = 16 / sizeof(T);
+  float best = -INFINITY;
   int done = 0;
   if (a.vec) {
     const int nv = n / kVec;
-    for (int i = threadIdx.x; i < nv; i += kThreads) {
-      uint4 x = __ldg(reinterpret_cast<const uint4*>(row) + i);
-      T* e = reinterpret_cast<T*>(&x);
+    constexpr int kAhead = 8;  // requests in flight per thread
+    for (int i0 = threadIdx.x; i0 < nv; i0 += kAhead * kThreads) {
+      uint4 x[kAhead];
 #pragma unroll
-      for (int q = 0; q < kVec; ++q) e[q] = take(i * kVec + q, e[q]);
-      reinterpret_cast<uint4*>(sl)[i] = x;
+      for (int j = 0; j < kAhead; ++j)
+        if (i0 + j * kThreads < nv) x[j] = __ldg(reinterpret_cast<const uint4*>(row) + i0 + j * kThreads);
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+        if (i0 + j * kThreads < nv) {
+          reinterpret_cast<uint4*>(sl)[i0 + j * kThreads] = x[j];
+          if constexpr (sizeof(T) == 2) {
+            const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&x[j]);
+            const __nv_bfloat162 m = __hmax2(__hmax2(e[0], e[1]), __hmax2(e[2], e[3]));
+            best = fmaxf(best, fmaxf(__low2float(m), __high2float(m)));
+          } else {
+            const float* e = reinterpret_cast<const float*>(&x[j]);
+            best = fmaxf(best, fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])));
+          }
+        }
     }
     done = nv * kVec;
   }
-  for (int i = done + threadIdx.x; i < chunks * kChunk; i += kThreads)
-    sl[i] = i < n ? take(i, row[i]) : static_cast<T>(-INFINITY);
-  auto better = [&](float v, int i) {
-    if (v > best || (v == best && i < arg)) best = v, arg = i;
-  };
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    better(__shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, arg, o));
-  if (lane == 0) s.red_f[w] = best, s.red_i[w] = arg;
+  for (int i = done + threadIdx.x; i < chunks * kChunk; i += kThreads) {
+    const T x = i < n ? row[i] : static_cast<T>(-INFINITY);
+    sl[i] = x;
+    best = fmaxf(best, to_float(x));
+  }
+  best = warp_max(best);
+  if (lane == 0) s.red_f[w] = best;
+  if (threadIdx.x == 0) s.n_list = 0;
   cl.sync();  // also: every CTA of the cluster runs, so its shared memory may be written
   if (threadIdx.x < C) {
-    for (int i = 0; i < kWarps; ++i) better(s.red_f[i], s.red_i[i]);
-    Shared* o = remote(cl, &s, threadIdx.x);
-    o->cl_max[me] = best;
-    o->cl_arg[me] = arg;
+    for (int i = 0; i < kWarps; ++i) best = fmaxf(best, s.red_f[i]);
+    remote(cl, &s, threadIdx.x)->cl_max[me] = best;
   }
   cl.sync();
-  for (int r = 0; r < C; ++r) better(s.cl_max[r], s.cl_arg[r]);
+  for (int r = 0; r < C; ++r) best = fmaxf(best, s.cl_max[r]);
 
-  const float t = a.temp[b];
   int* out = a.out + (long)b * a.draws;
-  if (!(t > 0.f) || best == -INFINITY) {  // greedy, or nothing to draw from
+  if (best == -INFINITY) {  // nothing to draw from (the whole cluster leaves; nothing of it is written any more)
     if (me == 0)
-      for (int d = threadIdx.x; d < a.draws; d += kThreads) out[d] = best == -INFINITY ? -1 : arg;
-    return;  // the whole cluster; nothing of it is written any more
+      for (int d = threadIdx.x; d < a.draws; d += kThreads) out[d] = -1;
+    return;
   }
-  // every thread holds the row's maximum: `best` of other warps saw all of cl_max too
+  if (!(t > 0.f)) {  // greedy: the first index of the maximum
+    int at = 0x7fffffff;
+    for_chunks(sl, chunks, [&](int i, const float(&v)[8]) {
+#pragma unroll
+      for (int e = 7; e >= 0; --e)
+        if (v[e] == best) at = min(at, s0 + i + e);
+    });
+    at = __reduce_min_sync(0xffffffffu, at);
+    if (lane == 0) s.red_a[w] = at;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < kWarps; ++i) at = min(at, static_cast<int>(s.red_a[i]));
+      remote(cl, &s, 0)->cl_arg[me] = at;
+    }
+    cl.sync();
+    if (me == 0) {
+      for (int r = 0; r < C; ++r) at = min(at, s.cl_arg[r]);
+      for (int d = threadIdx.x; d < a.draws; d += kThreads) out[d] = at;
+    }
+    return;
+  }
+  // the table of powers, from 2 x 32 of them
+  if (threadIdx.x < 64) {
+    const int j = threadIdx.x & 31;
+    s.tab[threadIdx.x] = threadIdx.x < 32 ? exp2(45.0 + j / 32.0) : exp2(j / 1024.0);
+  }
+  __syncthreads();
+  double pw[kTab / kThreads];
+#pragma unroll
+  for (int q = 0; q < kTab / kThreads; ++q) {
+    const int j = threadIdx.x + q * kThreads;
+    pw[q] = s.tab[j >> 5] * s.tab[32 + (j & 31)];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < kTab / kThreads; ++q) s.tab[threadIdx.x + q * kThreads] = pw[q];
+  if (best == INFINITY) {  // the limit of finite ones: infinities share the mass
+    for (int i = threadIdx.x; i < chunks * kChunk; i += kThreads)
+      sl[i] = static_cast<T>(to_float(sl[i]) == INFINITY ? 0.f : -INFINITY);
+    best = 0.f;
+  }
+  __syncthreads();
   Row r;
   r.mx = best;
-  r.mxd = best;
-  r.inv_t = 1.0 / static_cast<double>(t);
-  r.inv_tf = static_cast<float>(r.inv_t);
-  const float mp = a.min_p != nullptr ? a.min_p[b] : 0.f;
-  r.min_w = mp > 0.f ? fmin(1.0, static_cast<double>(mp)) : 0.0;
-  const int k = a.top_k != nullptr ? a.top_k[b] : 0;
-  const float p = a.top_p != nullptr ? a.top_p[b] : 1.f;
+  const double td = static_cast<double>(t);
+  r.c = 1477.3197218702985 / td;  // 1024 / ln 2
+  r.mxd = static_cast<double>(best);
+  r.bins = static_cast<float>(kBinsPerT / td);
+  r.low = fmaxf(static_cast<float>(static_cast<double>(best) - kRange * td), -FLT_MAX);
   const bool need_k = k > 0 && k < a.V, need_p = p > 0.f && p < 1.f;
-  Cut cut{0u, 0x7fffffff, 0ull};
+  Cut cut{r.low, 0x7fffffff};
   if (need_k || need_p) {
-    clear_hist(s);
+    clear_hist(s, true);
     __syncthreads();
-    for_chunks(sl, chunks, [&](int, int, const float(&v)[8]) {
+    for_chunks(sl, chunks, [&](int, const float(&v)[8]) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) hist_add(s, bin_of(v[e], r), need_p, need_p ? mass_of(v[e], r, s.tab) : 0);
+      for (int e = 0; e < 8; ++e)
+        if (v[e] >= r.low) atomicAdd(&s.h.cnt[bin_of(v[e], r)], 1u);
     });
-    combine(cl, s, 0);
-    u64 z = s.mass[0][kBins - 1];
-    if (need_k) {
-      cut = select(cl, s, sl, chunks, s0, r, 0, false, need_p, static_cast<u64>(k));
-      z = cut.mass;
+    combine(cl, s, 0, true, false);
+    unsigned total = s.count[0][kBins - 1];
+    if (need_k && static_cast<unsigned>(k) < total) {
+      const int bk = find(s, 0, static_cast<u64>(k));
+      const unsigned before = bk ? s.count[0][bk - 1] : 0, inside = s.count[0][bk] - before;
+      cut = inside <= kList
+                ? sort_select(cl, s, sl, chunks, s0, r, 0, cut, bk, inside, false, before, static_cast<u64>(k))
+                : narrow_select(cl, s, sl, chunks, s0, r, 0, cut, bk, inside, 0ull, false, before, 0ull,
+                                static_cast<u64>(k));
+      total = static_cast<unsigned>(k);
     }
     if (need_p) {
-      const u64 target = static_cast<u64>(ceil(static_cast<double>(p) * static_cast<double>(z)));
-      cut = select(cl, s, sl, chunks, s0, r, 1, true, true, target > 0 ? target : 1);
+      // Bounds on the inclusive masses: c_b e^-(b + 1)/32 <= mass of bin b <= c_b e^-b/32, with 1e-4 of room for the
+      // roundings of bins and sums.  `total` ends the counts where top-k does.
+      const int b0 = 2 * threadIdx.x;
+      double up[2], dn[2];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int i = b0 + q;
+        const unsigned prev = i ? min(s.count[0][i - 1], total) : 0, c = min(s.count[0][i], total) - prev;
+        const double e = exp2f(-static_cast<float>(i) * (1.4426950408889634f / kBinsPerT));
+        up[q] = c * e * 1.0001;
+        dn[q] = c * e * (0.96923323447634 * 0.9999);  // e^(-1/32)
+      }
+      double xu = up[0] + up[1], xd = dn[0] + dn[1];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double yu = __shfl_up_sync(0xffffffffu, xu, o), yd = __shfl_up_sync(0xffffffffu, xd, o);
+        if (lane >= o) xu += yu, xd += yd;
+      }
+      if (lane == 31) s.whi[w] = xu, s.wlo[w] = xd;
+      if (threadIdx.x == 0) s.found = 0, s.found2 = kBins - 1;
+      __syncthreads();
+      double bu = 0, bd = 0, zu = 0, zd = 0;
+      for (int i = 0; i < kWarps; ++i) {
+        if (i < w) bu += s.whi[i], bd += s.wlo[i];
+        zu += s.whi[i], zd += s.wlo[i];
+      }
+      // the cut's bin is the first whose mass reaches p Z: none whose upper bound is below the lowest p Z, and none
+      // after the first whose lower bound reaches the highest
+      const double pd = static_cast<double>(p);
+      xu += bu, xd += bd;
+#pragma unroll
+      for (int q = 1; q >= 0; --q) {
+        const double iu = q ? xu : xu - up[1], id = q ? xd : xd - dn[1];
+        if (iu >= pd * zd && iu - up[q] < pd * zd) s.found = b0 + q;
+        if (id >= pd * zu && id - dn[q] < pd * zu) s.found2 = b0 + q;
+      }
+      clear_hist(s, true);
+      __syncthreads();
+      const int wlo = static_cast<int>(s.found), whi = static_cast<int>(s.found2);
+      // exact masses: above the window, in the window by bins, and of all
+      u64 above = 0, all = 0;
+      const Cut in{cut.v, cut.last - s0};  // indexes within the slice
+      for_chunks(sl, chunks, [&](int i, const float(&v)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const bool keep = keeps(in, v[e], i + e);
+          const u64 m = mass_if(keep, v[e], r, s.tab);
+          const int q = bin_of(v[e], r);
+          all += m;
+          above += q < wlo ? m : 0;
+          if (keep && q >= wlo && q <= whi) hist_mass(s, q, m);
+        }
+      });
+      above = warp_sum_u64(above);
+      all = warp_sum_u64(all);
+      __syncthreads();  // wsum, whi are read no more
+      if (lane == 0) s.wsum[w] = above, reinterpret_cast<u64*>(s.whi)[w] = all;
+      __syncthreads();
+      if (threadIdx.x < C) {
+        above = all = 0;
+        for (int i = 0; i < kWarps; ++i) above += s.wsum[i], all += reinterpret_cast<u64*>(s.whi)[i];
+        Shared* o = remote(cl, &s, threadIdx.x);
+        o->cl_above[me] = above;
+        o->cl_all[me] = all;
+      }
+      combine(cl, s, 1, false, true);
+      u64 head = 0, z = 0;
+      for (int i = 0; i < C; ++i) head += s.cl_above[i], z += s.cl_all[i];
+      u64 target = static_cast<u64>(ceil(pd * static_cast<double>(z)));
+      if (target < 1) target = 1;
+      const int bp = min(max(find(s, -1, target > head ? target - head : 1), wlo), whi);
+      const unsigned before = bp ? min(s.count[0][bp - 1], total) : 0;
+      const unsigned inside = min(s.count[0][bp], total) - before;
+      const u64 mbefore = head + (bp ? s.mass[bp - 1] : 0), minside = s.mass[bp] - (bp ? s.mass[bp - 1] : 0);
+      if (inside > 0)
+        cut = inside <= kList ? sort_select(cl, s, sl, chunks, s0, r, 1, cut, bp, inside, true, mbefore, target)
+                              : narrow_select(cl, s, sl, chunks, s0, r, 1, cut, bp, inside, minside, true, before,
+                                              mbefore, target);
     }
   }
-  // mass of token `i` of the slice if it is kept
-  auto kept = [&](float v, int i) -> u64 {
-    const unsigned key = key_of(v);
-    if (key < cut.key || (key == cut.key && s0 + i > cut.last)) return 0;
-    const double x = weight(v, r, s.tab);
-    return x >= r.min_w ? fixed(x) : 0;
-  };
+  if (mp > 0.f) {  // values at or above max + t ln(min_p), as the smallest float that is
+    const double thr = static_cast<double>(best) + td * log(fmin(1.0, static_cast<double>(mp)));
+    float f = static_cast<float>(thr);
+    if (static_cast<double>(f) < thr) f = nextafterf(f, INFINITY);
+    if (f > cut.v) cut = Cut{f, 0x7fffffff};
+  }
+  const Cut in{cut.v, cut.last - s0};  // indexes within the slice
   // ---- sums of 256 tokens in vocabulary order
-  for_chunks(sl, chunks, [&](int c, int i, const float(&v)[8]) {
+  for_chunks(sl, chunks, [&](int i, const float(&v)[8]) {
+    bool some = false;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) some |= v[e] >= cut.v;
     u64 m = 0;
+    if (__any_sync(0xffffffffu, some)) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) m += kept(v[e], i + e);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
-    if (lane == 0) csum[c] = m;
+      for (int e = 0; e < 8; ++e) m += mass_if(keeps(in, v[e], i + e), v[e], r, s.tab);
+      m = warp_sum_u64(m);
+    }
+    if (lane == 0) csum[i / kChunk] = m;
   });
   __syncthreads();
-  if (w == 0) {  // inclusive scan of the chunk sums
+  if (w == 0) {  // inclusive scan of the sums
     u64 carry = 0;
     for (int c0 = 0; c0 < chunks; c0 += 32) {
       u64 x = c0 + lane < chunks ? csum[c0 + lane] : 0;
@@ -510,7 +725,8 @@ __global__ void __launch_bounds__(kThreads) draw_kernel(const Args a) {
     const int i = c0 * kChunk + lane * 8;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      m[e] = kept(clean<T>(sl[i + e]), i + e);
+      const float v = to_float(sl[i + e]);
+      m[e] = mass_if(keeps(in, v, i + e), v, r, s.tab);
       sum += m[e];
     }
     u64 incl = sum;

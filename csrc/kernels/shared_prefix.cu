@@ -399,7 +399,7 @@ struct Cfg {
   static constexpr int kRegion = kKv * 128;       // 64 dims of a K or V tile: token rows of 128 bytes
   static constexpr int kTile = kKv * D * 2;
   static constexpr int kQ = kRows * D * 2;
-  static constexpr int kStages = D == 128 ? 4 : 8;  // of the K ring and of the V ring
+  static constexpr int kStages = D == 128 ? 3 : 8;  // of the K ring and of the V ring
   static constexpr int kSmem = 2 * kQ + 2 * kStages * kTile + 512 + 1024;
 };
 
