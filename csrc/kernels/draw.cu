@@ -6,7 +6,7 @@
 //   min-p  keeps w_i >= min_p, i.e. l_i >= max + t ln(min_p)
 //   token  the first kept i in vocabulary order whose inclusive sum exceeds u Z_kept
 //
-// The token is a whole number, so sums decide it at borders: weights are computed in fp64 (error below 1e-11) and summed
+// The token is a whole number, so sums decide it at borders: weights are computed in fp64 (error below 1e-10) and summed
 // as 64-bit fixed point with 2^45 for the largest.  Integer sums are exact and do not depend on the order of atomics,
 // so a call gives the same tokens every time.  Weights below 2^-46 of the largest (32 t below the maximum) count as 0.
 //
@@ -47,7 +47,7 @@ constexpr int64_t kMaxVocab = 1 << 18;  // sums of 2^45 stay below 2^63
 constexpr int kMaxSliceBytes = 128 * 1024;
 constexpr float kRange = 32.f;       // in units of t below the maximum; e^-32 < 2^-46
 constexpr float kBinsPerT = kBins / kRange;
-constexpr int kTab = 1024;
+constexpr int kTab = 512;
 constexpr int kList = 2048;          // tokens that one CTA sorts
 
 using u64 = unsigned long long;
@@ -69,6 +69,7 @@ struct Args {
 
 struct Hist {
   unsigned cnt[kBins], lo[kBins], hi[kBins];  // this CTA's counts and masses
+  unsigned fine[kBins];                       // the cluster's counts of a finer level, scanned
 };
 // What top-k / top-p keep: values above `v`, and of those equal to it the ones at or before `last`.
 struct Cut {
@@ -76,12 +77,12 @@ struct Cut {
   int last;
 };
 struct Shared {
-  double tab[kTab];                    // 2^45 2^(j / 1024)
+  double tab[kTab];                    // 2^45 2^(j / 512)
   union {
     Hist h;
     u64 list[kList];                   // (order-preserving bits of the value, ~index)
   };
-  unsigned count[2][kBins];            // the cluster's counts, scanned: [0] first level, [1] the finer ones
+  unsigned count[kBins];               // the cluster's counts of the first level, scanned
   u64 mass[kBins];
   u64 wsum[kWarps];
   double wlo[kWarps], whi[kWarps];
@@ -99,6 +100,8 @@ struct Shared {
   unsigned red_a[kWarps], red_b[kWarps];
 };
 
+__device__ __forceinline__ unsigned* counts_of(Shared& s, int lv) { return lv == 0 ? s.count : s.h.fine; }
+
 // Order-preserving bits of a float (-0 as +0).
 __device__ __forceinline__ unsigned key_of(float v) {
   const unsigned b = __float_as_uint(v + 0.f);
@@ -111,20 +114,20 @@ __device__ __forceinline__ float value_of(unsigned key) {
 struct Row {
   float mx, bins;      // bins per unit of l
   float low;           // values below it have no mass
-  double mxd, c;       // the maximum, 1024 / (t ln 2)
+  double mxd, c;       // the maximum, 512 / (t ln 2)
 };
-// round(2^45 exp((l - max) / t)) for l >= low: y = 1024 (l - max) / (t ln 2) = n + f with n = 1024 k + j, then
-// 2^k 2^(j / 1024) e^(f ln 2 / 1024): a table of powers, and 1 + x + x^2 / 2 for |x| < 3.4e-4 (remainder < 7e-12).  The
+// round(2^45 exp((l - max) / t)) for l >= low: y = 512 (l - max) / (t ln 2) = n + f with n = 512 k + j, then
+// 2^k 2^(j / 512) e^(f ln 2 / 512): a table of powers, and 1 + x + x^2 / 2 for |x| < 6.8e-4 (remainder < 6e-11).  The
 // rounding to n adds 1.5 2^52, whose low bits are n; the rounding to a whole mass adds 2^52.
 __device__ __forceinline__ u64 mass_of(float l, const Row& r, const double* tab) {
-  constexpr double kMagic = 6755399441055744.0, a = 6.7690154351557157e-4;  // ln 2 / 1024
+  constexpr double kMagic = 6755399441055744.0, a = 1.3538030870311430e-3;  // ln 2 / 512
   const double y = (static_cast<double>(l) - r.mxd) * r.c;  // the difference is exact, or nearly: logits may be large
   const double z = y + kMagic;
   const int n = __double2loint(z);
   const double f = y - (z - kMagic);
   const double p = fma(f, fma(f, 0.5 * a * a, a), 1.0);
   const double v = tab[n & (kTab - 1)] * p;
-  const double w = __hiloint2double(__double2hiint(v) + ((n & ~(kTab - 1)) << 10), __double2loint(v));
+  const double w = __hiloint2double(__double2hiint(v) + ((n & ~(kTab - 1)) << 11), __double2loint(v));
   return static_cast<u64>(__double_as_longlong(w + 4503599627370496.0)) & 0xfffffffffffffull;
 }
 // What a cut keeps, for all values including those below low, and the mass then.  Without a branch: in one, a warp
@@ -211,14 +214,15 @@ __device__ void combine(cg::cluster_group& cl, Shared& s, int lv, bool counts, b
     }
     for (int r = 0; r < C; ++r) {
       Shared* o = remote(cl, &s, r);
-      if (counts) o->count[lv][b] = c;
+      if (counts) counts_of(*o, lv)[b] = c;
       if (masses) o->mass[b] = m;
     }
   }
   cl.sync();
   // block scan, two bins per thread
   const int lane = lane_id(), w = warp_id(), b0 = 2 * threadIdx.x;
-  const unsigned c0 = counts ? s.count[lv][b0] : 0, c1 = counts ? s.count[lv][b0 + 1] : 0;
+  unsigned* cs = counts_of(s, lv);
+  const unsigned c0 = counts ? cs[b0] : 0, c1 = counts ? cs[b0 + 1] : 0;
   const u64 m0 = masses ? s.mass[b0] : 0, m1 = masses ? s.mass[b0 + 1] : 0;
   unsigned c = c0 + c1;
   u64 m = m0 + m1;
@@ -234,7 +238,7 @@ __device__ void combine(cg::cluster_group& cl, Shared& s, int lv, bool counts, b
   u64 mb = 0;
   for (int i = 0; i < w; ++i) cb += s.wcnt[i], mb += s.wsum[i];
   c += cb, m += mb;
-  if (counts) s.count[lv][b0] = c - c1, s.count[lv][b0 + 1] = c;
+  if (counts) cs[b0] = c - c1, cs[b0 + 1] = c;
   if (masses) s.mass[b0] = m - m1, s.mass[b0 + 1] = m;
   __syncthreads();
 }
@@ -244,8 +248,8 @@ __device__ int find(Shared& s, int lv, u64 target) {
   if (threadIdx.x == 0) s.found = kBins - 1;
   __syncthreads();
   for (int b = threadIdx.x; b < kBins; b += kThreads) {
-    const u64 v = lv < 0 ? s.mass[b] : s.count[lv][b];
-    const u64 p = b == 0 ? 0 : lv < 0 ? s.mass[b - 1] : s.count[lv][b - 1];
+    const u64 v = lv < 0 ? s.mass[b] : counts_of(s, lv)[b];
+    const u64 p = b == 0 ? 0 : lv < 0 ? s.mass[b - 1] : counts_of(s, lv)[b - 1];
     if (v >= target && p < target) s.found = b;  // at most one bin
   }
   __syncthreads();
@@ -381,8 +385,8 @@ __device__ Cut narrow_select(cg::cluster_group& cl, Shared& s, const T* sl, int 
     });
     combine(cl, s, 1, true, by_mass);
     const int b = by_mass ? find(s, -1, target - mbefore) : find(s, 1, target - before);
-    const unsigned cb = b ? s.count[1][b - 1] : 0;
-    inside = s.count[1][b] - cb;
+    const unsigned cb = b ? s.h.fine[b - 1] : 0;
+    inside = s.h.fine[b] - cb;
     before += cb;
     if (by_mass) {
       const u64 mb = b ? s.mass[b - 1] : 0;
@@ -535,21 +539,14 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const Args a) {
     }
     return;
   }
-  // the table of powers, from 2 x 32 of them
-  if (threadIdx.x < 64) {
-    const int j = threadIdx.x & 31;
-    s.tab[threadIdx.x] = threadIdx.x < 32 ? exp2(45.0 + j / 32.0) : exp2(j / 1024.0);
-  }
+  // the table of powers, from 16 and 32 of them
+  static_assert(kTab == kThreads, "one entry per thread");
+  if (threadIdx.x < 48)
+    s.tab[threadIdx.x] = threadIdx.x < 16 ? exp2(45.0 + threadIdx.x / 16.0) : exp2((threadIdx.x - 16) / 512.0);
   __syncthreads();
-  double pw[kTab / kThreads];
-#pragma unroll
-  for (int q = 0; q < kTab / kThreads; ++q) {
-    const int j = threadIdx.x + q * kThreads;
-    pw[q] = s.tab[j >> 5] * s.tab[32 + (j & 31)];
-  }
+  const double pw = s.tab[threadIdx.x >> 5] * s.tab[16 + (threadIdx.x & 31)];
   __syncthreads();
-#pragma unroll
-  for (int q = 0; q < kTab / kThreads; ++q) s.tab[threadIdx.x + q * kThreads] = pw[q];
+  s.tab[threadIdx.x] = pw;
   if (best == INFINITY) {  // the limit of finite ones: infinities share the mass
     for (int i = threadIdx.x; i < chunks * kChunk; i += kThreads)
       sl[i] = static_cast<T>(to_float(sl[i]) == INFINITY ? 0.f : -INFINITY);
@@ -559,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const Args a) {
   Row r;
   r.mx = best;
   const double td = static_cast<double>(t);
-  r.c = 1477.3197218702985 / td;  // 1024 / ln 2
+  r.c = 738.65986093514926 / td;  // 512 / ln 2
   r.mxd = static_cast<double>(best);
   r.bins = static_cast<float>(kBinsPerT / td);
   r.low = fmaxf(static_cast<float>(static_cast<double>(best) - kRange * td), -FLT_MAX);
@@ -574,10 +571,10 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const Args a) {
         if (v[e] >= r.low) atomicAdd(&s.h.cnt[bin_of(v[e], r)], 1u);
     });
     combine(cl, s, 0, true, false);
-    unsigned total = s.count[0][kBins - 1];
+    unsigned total = s.count[kBins - 1];
     if (need_k && static_cast<unsigned>(k) < total) {
       const int bk = find(s, 0, static_cast<u64>(k));
-      const unsigned before = bk ? s.count[0][bk - 1] : 0, inside = s.count[0][bk] - before;
+      const unsigned before = bk ? s.count[bk - 1] : 0, inside = s.count[bk] - before;
       cut = inside <= kList
                 ? sort_select(cl, s, sl, chunks, s0, r, 0, cut, bk, inside, false, before, static_cast<u64>(k))
                 : narrow_select(cl, s, sl, chunks, s0, r, 0, cut, bk, inside, 0ull, false, before, 0ull,
@@ -592,7 +589,7 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const Args a) {
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         const int i = b0 + q;
-        const unsigned prev = i ? min(s.count[0][i - 1], total) : 0, c = min(s.count[0][i], total) - prev;
+        const unsigned prev = i ? min(s.count[i - 1], total) : 0, c = min(s.count[i], total) - prev;
         const double e = exp2f(-static_cast<float>(i) * (1.4426950408889634f / kBinsPerT));
         up[q] = c * e * 1.0001;
         dn[q] = c * e * (0.96923323447634 * 0.9999);  // e^(-1/32)
@@ -656,8 +653,8 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const Args a) {
       u64 target = static_cast<u64>(ceil(pd * static_cast<double>(z)));
       if (target < 1) target = 1;
       const int bp = min(max(find(s, -1, target > head ? target - head : 1), wlo), whi);
-      const unsigned before = bp ? min(s.count[0][bp - 1], total) : 0;
-      const unsigned inside = min(s.count[0][bp], total) - before;
+      const unsigned before = bp ? min(s.count[bp - 1], total) : 0;
+      const unsigned inside = min(s.count[bp], total) - before;
       const u64 mbefore = head + (bp ? s.mass[bp - 1] : 0), minside = s.mass[bp] - (bp ? s.mass[bp - 1] : 0);
       if (inside > 0)
         cut = inside <= kList ? sort_select(cl, s, sl, chunks, s0, r, 1, cut, bp, inside, true, mbefore, target)
