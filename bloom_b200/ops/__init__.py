@@ -558,14 +558,15 @@ class SharedPrefixPlan:
                  "num_kv_heads", "head_dim", "q_len")
 
 
-def _prefix_chunk(prefix, tiles, step: int, slots: int) -> int:
+def _prefix_chunk(prefix, tiles, step: int, slots: int, part: float) -> int:
     """Prefix tokens per split, the same for all groups: of the multiples of `step` the one that ends first when
-    `slots` CTAs run at a time and a CTA takes as long as its steps and two more (start-up, result)."""
+    `slots` CTAs run at a time, a CTA takes as long as its steps and four more (start-up, result), and each split costs
+    `part` steps for its partial result (written once, read once)."""
     most = max((-(-n // step) for n in prefix), default=1)
     best = None
     for c in range(max(1, -(-most // 64)), most + 1):  # at most 64 splits
         ctas = sum(t * -(-n // (c * step)) for t, n in zip(tiles, prefix))
-        cost = -(-ctas // slots) * (c + 2)
+        cost = -(-ctas // slots) * (c + 4) + part * -(-most // c)
         if best is None or cost < best[0]:
             best = (cost, c)
     return best[1] * step if best else step
@@ -599,7 +600,9 @@ def shared_prefix_plan(group_sizes, prefix_lens, *, num_q_heads: int, num_kv_hea
     p.tile_rows = next((t for t in (8, 16, 32, 128) if most <= t), 256)
     tiles = [-(-r // p.tile_rows) for r in rows]
     step, slots = (64, 2 * sms) if p.tile_rows <= 32 else (128 if p.tile_rows == 256 else 256, sms)
-    chunk = _prefix_chunk(prefix, [t * num_kv_heads for t in tiles], step, slots)
+    # a step takes about 2 us, partial results (through L2) move at about 10 MB/us
+    part = sum(sizes) * q_len * num_q_heads * head_dim * 8 * (2 if p.tile_rows == 128 else 1) / 1e7 / 2
+    chunk = _prefix_chunk(prefix, [t * num_kv_heads for t in tiles], step, slots, part)
     items, groups, seqs = [], [], []
     p.prefix_splits = 1
     first = 0
@@ -639,7 +642,7 @@ def shared_prefix_attention(q, kv_cache, layer, block_table, seq_lens, out, *, p
     _C().shared_prefix_attention(q, kv_cache, layer, block_table, seq_lens, out, plan.items, plan.groups,
                                  plan.seqs, plan.q_len, plan.tile_rows, plan.prefix_splits, plan.suffix_splits,
                                  scale)
-    _count(2 if plan.items.shape[0] else 1)
+    _count(1 if not plan.items.shape[0] else 2 if plan.tile_rows <= 128 else 3)
     return out
 
 

@@ -27,6 +27,7 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cfloat>
 
 #include "bloom/common.cuh"
@@ -751,7 +752,14 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const Args a) {
 template <typename T>
 void launch(const Args& a, int B, int C, cudaStream_t stream) {
   const int smem = int((sizeof(Shared) + 15) / 16 * 16 + a.slice * sizeof(T) + a.slice / kChunk * sizeof(u64));
-  C10_CUDA_CHECK(cudaFuncSetAttribute(draw_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  static std::atomic<uint64_t> configured{0};  // per device: the limit of dynamic shared memory has been raised
+  int dev = 0;
+  C10_CUDA_CHECK(cudaGetDevice(&dev));
+  if (!(configured.load(std::memory_order_acquire) >> dev & 1u)) {
+    constexpr int most = int((sizeof(Shared) + 15) / 16 * 16 + kMaxSliceBytes + kMaxSliceBytes / sizeof(T) / kChunk * sizeof(u64));
+    C10_CUDA_CHECK(cudaFuncSetAttribute(draw_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    configured.fetch_or(uint64_t(1) << dev, std::memory_order_release);
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(B) * C);
   cfg.blockDim = dim3(kThreads);

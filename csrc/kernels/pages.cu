@@ -220,6 +220,7 @@ __device__ __forceinline__ int2 block_exscan2(int2 v, int2* warp_sums, int2& tot
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const CompactArgs a) {
   extern __shared__ uint32_t held[];
   __shared__ int2 sums[32];
+  griddep_launch_dependents();
   const int t = threadIdx.x, lane = t & 31;
   const int words = (a.NB + 31) / 32;
   int mine = 0;
@@ -439,15 +440,23 @@ std::tuple<torch::Tensor, torch::Tensor> kv_compact(torch::Tensor& kv_cache, tor
   a.n_moves = a.dst + half;
   a.status = status_word(kv_cache.get_device());
   const int smem = (NB + 31) / 32 * 4;
-  if (smem > 48 * 1024)
-    C10_CUDA_CHECK(cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (smem > 48 * 1024)  // pools of more than 393,216 pages
+    C10_CUDA_CHECK(cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxPages / 8));
   plan_kernel<<<1, kPlanThreads, smem, stream>>>(a);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   // no more copy CTAs than there can be chunks, and at most 8 per SM
   const long most = std::max<long>(1, (long)(NB / 2) * a.L * a.chunks);
   const int copiers = int(std::min<long>(most, 8L * num_sms(kv_cache.get_device())));
-  move_kernel<<<unsigned(a.S + copiers), kThreads, 0, stream>>>(a);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  cudaLaunchConfig_t cfg = {};  // a dependent launch: its CTAs are there when the plan is done
+  cfg.gridDim = dim3(unsigned(a.S + copiers));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, move_kernel, a));
   return {moved, used};
 }
 

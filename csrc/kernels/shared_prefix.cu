@@ -7,19 +7,21 @@
 // o = (o1 2^(m1-M) + o2 2^(m2-M)) / (l1 2^(m1-M) + l2 2^(m2-M)).  So the prefix of a group is read once for all of its
 // members, as a product with members x q_len x (q heads per KV head) rows, and only the rest is read per sequence.
 //
-// Two kernels.  The prefix kernel (work items: a tile of a group's rows x a range of the prefix) leaves partial sums in
-// fp32.  The suffix kernel is one CTA (or a cluster over the pages) per sequence, KV head and chunk of rows; it is
-// launched as a dependent of the prefix kernel, runs its own pages beside it, and waits for it only before it adds the
-// partial sums and writes the result: two launches, memory and tensor work overlapped.
+// The prefix kernel (work items: a tile of a group's rows x a range of the prefix) leaves partial sums in fp32, the
+// suffix kernel is one CTA (or several over the pages) per sequence, KV head and chunk of rows.  Groups of few rows:
+// two launches, the suffix kernel a dependent of the prefix kernel that adds the parts at its end.  Groups of many rows,
+// whose prefix is work for the tensor cores: both side by side on two streams, and a third kernel adds the parts.
 //
 // Slots behind a sequence's last token may hold anything (NaN too): scores there are replaced, and V rows there are
 // zeroed in shared memory.  A block id outside the cache sets kStatusBadArgument and page 0 is read instead.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/CUDAEvent.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cooperative_groups.h>
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "bloom/common.cuh"
 #include "bloom/ops_share.h"
@@ -142,7 +144,7 @@ int stream_smem(int warps, int rows) {
 // m16n8k16 and 4 to 8 query rows (a GQA group) fill its 8-column side: half the MMAs and half the registers for O of
 // the other way round.  P^T moves from accumulator to B fragments by an 8x8 transpose of the warp.  Each warp takes
 // every warps-th page through its own TMA ring.  (Loading fragments straight into registers needs no barriers, but
-// keeps only a page per warp in flight, and at 128 registers spills: 79 us where the rings take XX us for 268 MB of
+// keeps only a page per warp in flight, and at 128 registers spills: 79 us where the rings take 62 us for 268 MB of
 // 2,048 short sequences x heads.)
 template <int D, int NT, typename Limit>
 __device__ float* stream(const CUtensorMap& tm, const Args& a, uint8_t* smem, int* abort_flag, const int* row, int kh,
@@ -394,13 +396,15 @@ constexpr int kThreads = 256 + 32 + 64;
 constexpr int kTmemCols = 512;
 constexpr float kLazy = 8.f;  // log2 units
 
-template <int D>
+template <int D, bool kPair>
 struct Cfg {
   static constexpr int kRegion = kKv * 128;       // 64 dims of a K or V tile: token rows of 128 bytes
   static constexpr int kTile = kKv * D * 2;
   static constexpr int kQ = kRows * D * 2;
-  static constexpr int kStages = D == 128 ? 3 : 8;  // of the K ring and of the V ring
-  static constexpr int kSmem = 2 * kQ + 2 * kStages * kTile + 512 + 1024;
+  // of the K ring and of the V ring: one row tile waits for memory, two for the tensor cores, and leave room for CTAs
+  // of the suffix kernel
+  static constexpr int kStages = D == 64 ? 8 : kPair ? 2 : 5;
+  static constexpr int kSmem = (kPair ? 2 : 1) * kQ + 2 * kStages * kTile + 512 + 1024;
 };
 
 __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
@@ -472,13 +476,13 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t smem_addr, uint32_t lbo) {
 template <int D, bool kPair>
 __global__ void __launch_bounds__(kThreads, 1)
     prefix_tc_kernel(const __grid_constant__ CUtensorMap tm, const Args a) {
-  griddep_launch_dependents();
-  using C = Cfg<D>;
+  if constexpr (!kPair) griddep_launch_dependents();
+  using C = Cfg<D, kPair>;
   constexpr int kStages = C::kStages;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;
-  uint8_t* sK = smem + 2 * C::kQ;
+  uint8_t* sK = smem + (kPair ? 2 : 1) * C::kQ;
   uint8_t* sV = sK + kStages * C::kTile;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sV + kStages * C::kTile);
   uint64_t *fullK = bars, *emptyK = bars + 8, *fullV = bars + 16, *emptyV = bars + 24;
@@ -811,68 +815,38 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 }  // namespace tc
 
-// Each sequence's own keys, then the sum with the prefix.  grid (B, KV heads x row chunks, page splits), the splits of
-// a row one cluster.
-template <int D, int NT>
-__global__ void __launch_bounds__(kMaxWarps * 32) 
-    suffix_kernel(const __grid_constant__ CUtensorMap tm, const Args a, int row_chunks) {
-  extern __shared__ uint8_t raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  __shared__ int abort_flag;
-  if (threadIdx.x == 0) abort_flag = 0;
-  __syncthreads();
-  const int b = blockIdx.x, kh = blockIdx.y / row_chunks, r0 = blockIdx.y % row_chunks * (NT * 8);
-  const int G = a.nq / a.nkv, rows = min(NT * 8, a.ql * G - r0);
-  const int splits = gridDim.z, me = blockIdx.z;
-  const int2 sh = __ldg(a.seqs + b);
-  const int len = seq_len(a, b);
-  // this CTA's pages of [prefix, len)
-  const int begin = min(sh.x, len), p0 = begin / PAGE, pages = (len + PAGE - 1) / PAGE - p0;
-  const int per = (pages + splits - 1) / splits;
-  const int k0 = max(begin, (p0 + me * per) * PAGE), k1 = min(len, (p0 + (me + 1) * per) * PAGE);
-  float* res = stream<D, NT>(tm, a, smem, &abort_flag, a.table + (long)b * a.table_stride, kh, (long)b * a.ql, r0, rows,
-                             min(k0, max(k1, 0)), k1, [&](int r) { return len - a.ql + div_g(a, r0 + r); });
-  constexpr int RS = D + 2;
-  cg::cluster_group cl = cg::this_cluster();
-  if (splits > 1) cl.sync();
-  griddep_wait();
-  const int n_prefix = sh.y * a.parts;
-  // one warp per row, part s of the prefix in lane s & 31; the rows are dealt over the CTAs of the cluster
-  const int warps = blockDim.x / 32;
-  for (int r = me * warps + warp_id(); r < rows; r += splits * warps) {
+// Running sum over partial results of one row (a warp; lane `lane` holds dims lane * D / 32 ...).
+template <int D>
+struct RowSum {
+  float M = kNegBig, L = 0.f, O[D / 32] = {};
+
+  __device__ __forceinline__ void scale_to(float m) {
+    const float m_new = fmaxf(M, m), f = exp2f(M - m_new);
+    M = m_new;
+    L *= f;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) O[c] *= f;
+  }
+  // one part: O[D], m, l at p
+  __device__ __forceinline__ void add(const float* p) {
+    scale_to(p[D]);
+    const float w = exp2f(p[D] - M);
+    L += p[D + 1] * w;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) O[c] += p[lane_id() * (D / 32) + c] * w;
+  }
+  // n parts of the workspace, `step` rows apart, part s in lane s & 31
+  __device__ __forceinline__ void add_parts(const Args& a, long at, long step, int n) {
     const int lane = lane_id();
-    const int qi = div_g(a, r0 + r);
-    const long tok = (long)b * a.ql + qi;
-    const int h = kh * G + (r0 + r - qi * G);
-    const long at0 = tok * a.nq + h, step = (long)a.B * a.ql * a.nq;
-    float M = kNegBig, L = 0.f, O[D / 32];
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) O[c] = 0.f;
-    // adds a part (m, l, O / this lane's dims) to the running sum
-    auto scale_to = [&](float m) {
-      const float m_new = fmaxf(M, m), f = exp2f(M - m_new);
-      M = m_new;
-      L *= f;
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) O[c] *= f;
-    };
-    for (int s = 0; s < splits; ++s) {
-      const float* p = (splits > 1 ? cl.map_shared_rank(res, s) : res) + r * RS;
-      scale_to(p[D]);
-      const float w = exp2f(p[D] - M);
-      L += p[D + 1] * w;
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) O[c] += p[lane * (D / 32) + c] * w;
-    }
-    for (int s0 = 0; s0 < n_prefix; s0 += 32) {
-      const int n = min(32, n_prefix - s0);
-      const float2 ml = lane < n ? a.part_ml[at0 + (s0 + lane) * step] : make_float2(kNegBig, 0.f);
+    for (int s0 = 0; s0 < n; s0 += 32) {
+      const int k = min(32, n - s0);
+      const float2 ml = lane < k ? a.part_ml[at + (s0 + lane) * step] : make_float2(kNegBig, 0.f);
       scale_to(warp_max(ml.x));
       const float w = exp2f(ml.x - M);
       L += warp_sum(ml.y * w);
-      const float* p = a.part_o + (at0 + s0 * step) * D + lane * (D / 32);
+      const float* p = a.part_o + (at + s0 * step) * D + lane * (D / 32);
 #pragma unroll 4
-      for (int s = 0; s < n; ++s, p += step * D) {
+      for (int s = 0; s < k; ++s, p += step * D) {
         const float ws = __shfl_sync(0xffffffffu, w, s);
         if constexpr (D == 128) {
           const float4 v = *reinterpret_cast<const float4*>(p);
@@ -883,48 +857,133 @@ __global__ void __launch_bounds__(kMaxWarps * 32)
         }
       }
     }
+  }
+  __device__ __forceinline__ void store(const Args& a, long tok, int h) const {
     const float inv = L > 0.f ? 1.f / L : 0.f;  // a row that sees nothing gives zeros
-    __nv_bfloat16* dst = a.out + tok * a.out_stride + h * D + lane * (D / 32);
+    __nv_bfloat16* dst = a.out + tok * a.out_stride + h * D + lane_id() * (D / 32);
     if constexpr (D == 128)
       *reinterpret_cast<uint2*>(dst) =
           make_uint2(pack_bf16x2(O[0] * inv, O[1] * inv), pack_bf16x2(O[2] * inv, O[3] * inv));
     else
       *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(O[0] * inv, O[1] * inv);
   }
-  if (splits > 1) cl.sync();  // the others may still read this CTA's result
+};
+
+// Each sequence's own keys.  grid (B, KV heads x row chunks, page splits).
+// kMerge: a dependent of the prefix kernel, the splits of a row one cluster; adds the prefix's parts and writes the
+// result.  Otherwise it runs beside the prefix kernel, and its results are parts `first_part` ... of the workspace.
+template <int D, int NT, bool kMerge>
+__global__ void __launch_bounds__(kMaxWarps * 32)
+    suffix_kernel(const __grid_constant__ CUtensorMap tm, const Args a, int row_chunks, int first_part) {
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  __shared__ int abort_flag;
+  if (threadIdx.x == 0) abort_flag = 0;
+  __syncthreads();
+  const int b = blockIdx.x, kh = blockIdx.y / row_chunks, r0 = blockIdx.y % row_chunks * (NT * 8);
+  const int G = a.nq / a.nkv, rows = min(NT * 8, a.ql * G - r0);
+  const int splits = gridDim.z, me = blockIdx.z, warps = blockDim.x / 32;
+  const int2 sh = __ldg(a.seqs + b);
+  const int len = seq_len(a, b);
+  // this CTA's pages of [prefix, len)
+  const int begin = min(sh.x, len), p0 = begin / PAGE, pages = (len + PAGE - 1) / PAGE - p0;
+  const int per = (pages + splits - 1) / splits;
+  const int k0 = max(begin, (p0 + me * per) * PAGE), k1 = min(len, (p0 + (me + 1) * per) * PAGE);
+  float* res = stream<D, NT>(tm, a, smem, &abort_flag, a.table + (long)b * a.table_stride, kh, (long)b * a.ql, r0, rows,
+                             min(k0, max(k1, 0)), k1, [&](int r) { return len - a.ql + div_g(a, r0 + r); });
+  constexpr int RS = D + 2;
+  const long step = (long)a.B * a.ql * a.nq;
+  auto row_of = [&](int r, long& tok, int& h) {
+    const int qi = div_g(a, r0 + r);
+    tok = (long)b * a.ql + qi;
+    h = kh * G + (r0 + r - qi * G);
+  };
+  if constexpr (kMerge) {
+    cg::cluster_group cl = cg::this_cluster();
+    if (splits > 1) cl.sync();
+    griddep_wait();
+    // one warp per row, the rows dealt over the CTAs of the cluster
+    for (int r = me * warps + warp_id(); r < rows; r += splits * warps) {
+      long tok;
+      int h;
+      row_of(r, tok, h);
+      RowSum<D> sum;
+      for (int s = 0; s < splits; ++s) sum.add((splits > 1 ? cl.map_shared_rank(res, s) : res) + r * RS);
+      sum.add_parts(a, tok * a.nq + h, step, sh.y * a.parts);
+      sum.store(a, tok, h);
+    }
+    if (splits > 1) cl.sync();  // the others may still read this CTA's result
+  } else {
+    for (int r = warp_id(); r < rows; r += warps) {
+      long tok;
+      int h;
+      row_of(r, tok, h);
+      const long at = (first_part + me) * step + tok * a.nq + h;
+      const float* p = res + r * RS;
+#pragma unroll
+      for (int c = lane_id(); c < D; c += 32) a.part_o[at * D + c] = p[c];
+      if (lane_id() == 0) a.part_ml[at] = make_float2(p[D], p[D + 1]);
+    }
+  }
+}
+
+// The sum of all parts, one warp per row: the prefix's, and `own` of each sequence from `first_part` on.
+template <int D>
+__global__ void __launch_bounds__(256) merge_kernel(const Args a, int first_part, int own) {
+  const long row = (long)blockIdx.x * 8 + warp_id(), step = (long)a.B * a.ql * a.nq;
+  if (row >= step) return;
+  const long tok = row / a.nq;
+  RowSum<D> sum;
+  sum.add_parts(a, row, step, __ldg(a.seqs + tok / a.ql).y * a.parts);
+  sum.add_parts(a, row + first_part * step, step, own);
+  sum.store(a, tok, int(row - tok * a.nq));
+}
+
+// Raises a kernel's limit of dynamic shared memory once per device.
+template <typename K>
+void allow_smem(K* kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  C10_CUDA_CHECK(cudaGetDevice(&dev));
+  if (done.load(std::memory_order_acquire) >> dev & 1u) return;
+  C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  // all of an SM's memory as shared memory, also where one CTA of this kernel needs less: CTAs of another come beside it
+  C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                      cudaSharedmemCarveoutMaxShared));
+  done.fetch_or(uint64_t(1) << dev, std::memory_order_release);
 }
 
 template <int D, int NT>
 void launch_prefix(const CUtensorMap& tm, const Args& a, int items, cudaStream_t stream) {
   constexpr int kWarps = 4;
   const int smem = stream_smem<D>(kWarps, NT * 8);
-  C10_CUDA_CHECK(
-      cudaFuncSetAttribute(prefix_stream_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  static std::atomic<uint64_t> done{0};
+  allow_smem(prefix_stream_kernel<D, NT>, smem, done);
   prefix_stream_kernel<D, NT><<<dim3(items, a.nkv), kWarps * 32, smem, stream>>>(tm, a);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
 template <int D, bool kPair>
 void launch_prefix_tc(const CUtensorMap& tm, const Args& a, int items, cudaStream_t stream) {
-  constexpr int smem = tc::Cfg<D>::kSmem;
-  C10_CUDA_CHECK(
-      cudaFuncSetAttribute(tc::prefix_tc_kernel<D, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  constexpr int smem = tc::Cfg<D, kPair>::kSmem;
+  static std::atomic<uint64_t> done{0};
+  allow_smem(tc::prefix_tc_kernel<D, kPair>, smem, done);
   tc::prefix_tc_kernel<D, kPair><<<dim3(items, a.nkv), tc::kThreads, smem, stream>>>(tm, a);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
-template <int D, int NT>
-void launch_suffix(const CUtensorMap& tm, const Args& a, int splits, bool dependent, int sms, cudaStream_t stream) {
+template <int D, int NT, bool kMerge>
+void launch_suffix(const CUtensorMap& tm, const Args& a, int splits, int first_part, bool dependent, int sms,
+                   cudaStream_t stream) {
   const int row_chunks = (a.ql * (a.nq / a.nkv) + NT * 8 - 1) / (NT * 8);
   // Warps per sequence, KV head and row chunk: as many as fill the SMs once.  Each warp costs its start and its share
-  // of the merge, so where there are sequences enough one warp takes a whole one: 256 sequences x 8 heads of 1 to 511
-  // tokens took 79 us with four warps each, XX us with one.
+  // of the merge, and its ring the place of another CTA, so where there are sequences enough one warp takes a whole one:
+  // 256 sequences x 8 heads of 64 tokens take 14 us with one warp each, 26 with four; of 256 tokens 47 and 54.
   const long ctas = (long)a.B * a.nkv * row_chunks * splits;
   int warps = 1;
   while (warps * 2 <= kMaxWarps && ctas * warps * 2 <= (long)sms * kMaxWarps) warps *= 2;
   const int smem = stream_smem<D>(warps, std::min(NT * 8, a.ql * (a.nq / a.nkv)));
-  C10_CUDA_CHECK(cudaFuncSetAttribute(suffix_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      stream_smem<D>(kMaxWarps, NT * 8)));
+  static std::atomic<uint64_t> done{0};
+  allow_smem(suffix_kernel<D, NT, kMerge>, stream_smem<D>(kMaxWarps, NT * 8), done);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.B, a.nkv * row_chunks, splits);
   cfg.blockDim = dim3(warps * 32);
@@ -932,7 +991,7 @@ void launch_suffix(const CUtensorMap& tm, const Args& a, int splits, bool depend
   cfg.stream = stream;
   cudaLaunchAttribute at[2];
   int n = 0;
-  if (splits > 1) {
+  if (kMerge && splits > 1) {
     at[n].id = cudaLaunchAttributeClusterDimension;
     at[n].val.clusterDim.x = at[n].val.clusterDim.y = 1;
     at[n++].val.clusterDim.z = splits;
@@ -943,23 +1002,46 @@ void launch_suffix(const CUtensorMap& tm, const Args& a, int splits, bool depend
   }
   cfg.attrs = at;
   cfg.numAttrs = n;
-  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, suffix_kernel<D, NT>, tm, a, row_chunks));
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, suffix_kernel<D, NT, kMerge>, tm, a, row_chunks, first_part));
+}
+
+template <int D, bool kMerge>
+void run_suffix(const CUtensorMap& tm, const Args& a, int splits, int first_part, bool dependent, int sms,
+                cudaStream_t stream) {
+  const int rows = a.ql * (a.nq / a.nkv);
+  if (rows <= 8) launch_suffix<D, 1, kMerge>(tm, a, splits, first_part, dependent, sms, stream);
+  else if (rows <= 16) launch_suffix<D, 2, kMerge>(tm, a, splits, first_part, dependent, sms, stream);
+  else launch_suffix<D, 4, kMerge>(tm, a, splits, first_part, dependent, sms, stream);
 }
 
 template <int D>
-void run(const CUtensorMap& tm, const Args& a, int items, int tile_rows, int suffix_splits, int sms,
-         cudaStream_t stream) {
-  if (items > 0) {
-    if (tile_rows == 8) launch_prefix<D, 1>(tm, a, items, stream);
-    else if (tile_rows == 16) launch_prefix<D, 2>(tm, a, items, stream);
-    else if (tile_rows == 32) launch_prefix<D, 4>(tm, a, items, stream);
-    else if (tile_rows == 128) launch_prefix_tc<D, false>(tm, a, items, stream);
-    else launch_prefix_tc<D, true>(tm, a, items, stream);
+void run(const CUtensorMap& tm, const Args& a, int items, int tile_rows, int prefix_parts, int suffix_splits, int sms,
+         c10::cuda::CUDAStream stream) {
+  if (tile_rows <= 128 || items == 0) {
+    if (items > 0) {
+      if (tile_rows == 8) launch_prefix<D, 1>(tm, a, items, stream);
+      else if (tile_rows == 16) launch_prefix<D, 2>(tm, a, items, stream);
+      else if (tile_rows == 32) launch_prefix<D, 4>(tm, a, items, stream);
+      else launch_prefix_tc<D, false>(tm, a, items, stream);
+    }
+    run_suffix<D, true>(tm, a, suffix_splits, 0, items > 0, sms, stream);
+    return;
   }
-  const int rows = a.ql * (a.nq / a.nkv);
-  if (rows <= 8) launch_suffix<D, 1>(tm, a, suffix_splits, items > 0, sms, stream);
-  else if (rows <= 16) launch_suffix<D, 2>(tm, a, suffix_splits, items > 0, sms, stream);
-  else launch_suffix<D, 4>(tm, a, suffix_splits, items > 0, sms, stream);
+  // The prefix on the tensor cores and the suffixes from HBM run side by side on two streams.  (As a dependent launch
+  // the suffix kernel starts as early, but its wait for the prefix kernel does not end while its CTAs load: 119 us for
+  // 256 sequences behind 8,192 tokens, 108 this way; 120 and 103 for 16 groups of 8 that verify four tokens.  With one
+  // row tile the prefix is short, and the third launch costs more than it gives: 28 us and 30.)
+  const c10::cuda::CUDAStream side = at::cuda::getStreamFromPool(false, stream.device_index());
+  at::cuda::CUDAEvent fork, join;
+  fork.record(stream);
+  fork.block(side);
+  launch_prefix_tc<D, true>(tm, a, items, stream);
+  run_suffix<D, false>(tm, a, suffix_splits, prefix_parts, false, sms, side);
+  join.record(side);
+  join.block(stream);
+  const long rows = (long)a.B * a.ql * a.nq;
+  merge_kernel<D><<<unsigned((rows + 7) / 8), 256, 0, stream>>>(a, prefix_parts, suffix_splits);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
 }  // namespace shared_prefix
@@ -1011,7 +1093,7 @@ void shared_prefix_attention(const torch::Tensor& q, const torch::Tensor& kv_cac
     SP_CHECK(t->device() == q.device(), "tensors must be on one device");
   if (B == 0) return;
   const at::cuda::CUDAGuard guard(q.device());
-  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  const c10::cuda::CUDAStream stream = at::cuda::getCurrentCUDAStream();
   const int64_t T = B * q_len, nq = q.size(1);
   Args a;
   a.q = reinterpret_cast<const __nv_bfloat16*>(q.data_ptr());
@@ -1036,16 +1118,16 @@ void shared_prefix_attention(const torch::Tensor& q, const torch::Tensor& kv_cac
   a.scale_log2 = float(scale * 1.4426950408889634);
   a.status = status_word(q.get_device());
   a.parts = tile_rows == 128 ? 2 : 1;
-  prefix_splits *= a.parts;
-  // partial sums of the prefix: every (split, row) that the suffix kernel reads is written by an item
-  auto ws = torch::empty({prefix_splits * T * nq * (D + 2)}, q.options().dtype(at::kFloat));
+  // partial results: every (part, row) that is read has been written, the prefix's by the plan's items
+  const int64_t prefix_parts = prefix_splits * a.parts, parts = prefix_parts + (tile_rows == 256 ? suffix_splits : 0);
+  auto ws = torch::empty({parts * T * nq * (D + 2)}, q.options().dtype(at::kFloat));
   a.part_o = ws.data_ptr<float>();
-  a.part_ml = reinterpret_cast<float2*>(a.part_o + prefix_splits * T * nq * D);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + parts * T * nq * D);
   const auto* base = reinterpret_cast<const __nv_bfloat16*>(kv_cache.data_ptr()) + layer * kv_cache.stride(0);
   const CUtensorMap tm = make_tmap_bf16_2d(base, D, rows, D * 2, 64, PAGE);
   const int sms = num_sms(q.get_device());
-  if (D == 128) run<128>(tm, a, int(items.size(0)), int(tile_rows), int(suffix_splits), sms, stream);
-  else run<64>(tm, a, int(items.size(0)), int(tile_rows), int(suffix_splits), sms, stream);
+  if (D == 128) run<128>(tm, a, int(items.size(0)), int(tile_rows), int(prefix_parts), int(suffix_splits), sms, stream);
+  else run<64>(tm, a, int(items.size(0)), int(tile_rows), int(prefix_parts), int(suffix_splits), sms, stream);
 }
 
 }  // namespace bloom
