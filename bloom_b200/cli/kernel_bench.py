@@ -413,6 +413,61 @@ def main():
         ms = timeit(lambda i=0: ops.sample(logits, temp, topp, topk, seeds, offs, draft))
         report("verify_sample", ms, None, logits.numel() * 2, {"rows": R})
 
+    if not args.only or "share" in args.only:
+        # sequences that share a prompt: one layer of decode attention (groups x members behind a prefix, own tokens
+        # each), forking a batch, compacting a pool, drawing tokens from given uniforms
+        for groups, members, prefix, tail in ((1, 4, 512, 16), (1, 32, 4096, 128), (16, 8, 2048, 128),
+                                              (1, 256, 8192, 256)):
+            B, pp, tp = groups * members, prefix // 16, tail // 16
+            nb = groups * pp + B * tp
+            perm = torch.randperm(nb, device=dev, dtype=torch.int32)
+            head = perm[:groups * pp].view(groups, pp).repeat_interleave(members, 0)
+            table = torch.cat([head, perm[groups * pp:].view(B, tp)], 1).contiguous()
+            kv = torch.randn(1, nb, 2, nkv, 16, hd, device=dev, dtype=torch.bfloat16)
+            lens = torch.full((B,), prefix + tail, dtype=torch.int32, device=dev)
+            q = torch.randn(B, nq, hd, device=dev, dtype=torch.bfloat16)
+            out = torch.empty_like(q)
+            plan = ops.shared_prefix_plan([members] * groups, [prefix] * groups, num_q_heads=nq, num_kv_heads=nkv,
+                                          head_dim=hd, max_seq_len=prefix + tail, device=dev)
+            ex = {"groups": groups, "members": members, "prefix": prefix, "own": tail}
+            ms = timeit(lambda i=0: ops.shared_prefix_attention(q, kv, 0, table, lens, out, plan=plan,
+                                                                scale=hd ** -0.5))
+            report("shared_prefix_attention", ms, 4.0 * B * (prefix + tail) * nq * hd, nb * 2 * nkv * 16 * hd * 2, ex)
+            ms = timeit(lambda i=0: ops.paged_decode_attention(q, kv, 0, table, lens, out, scale=hd ** -0.5))
+            report("paged_decode_attention_same_tables", ms, 4.0 * B * (prefix + tail) * nq * hd,
+                   B * (prefix + tail) * 2 * nkv * hd * 2, ex)
+        C, n = 128, 1000
+        kv = torch.randn(8, 16 * 63 + C, 2, nkv, 16, hd, device=dev, dtype=torch.bfloat16)
+        table = torch.arange(16 * 63, device=dev, dtype=torch.int32).view(16, 63)
+        ref = torch.ones(16 * 63 + C, device=dev, dtype=torch.int32)
+        lens = torch.full((16,), n, dtype=torch.int32, device=dev)
+        parents = torch.arange(C, device=dev, dtype=torch.int32) // 8
+        fresh = torch.arange(16 * 63, 16 * 63 + C, device=dev, dtype=torch.int32)
+
+        def fork(i=0):
+            ref[16 * 63:].zero_()
+            ops.kv_fork(kv, table, lens, parents, fresh, ref)
+
+        report("kv_fork", timeit(fork), None, (16 + C) * 8 * kv.stride(1) * 2, {"children": C, "layers": 8})
+        kv = torch.randn(2, 8192, 2, nkv, 16, hd, device=dev, dtype=torch.bfloat16)
+        held = (torch.arange(8192, device=dev) % 2).int()  # every second page: half of the held ones move
+        none = torch.zeros(1, 1, dtype=torch.int32, device=dev)
+        ref = held.clone()
+
+        def compact(i=0):
+            ref.copy_(held)
+            ops.kv_compact(kv, none, none[0], ref)
+
+        report("kv_compact", timeit(compact), None, 2 * 2048 * 2 * kv.stride(1) * 2, {"pages": 8192, "layers": 2})
+        for B in (1, 256):
+            lg = torch.randn(B, V, device=dev, dtype=torch.bfloat16) * 3
+            u, tt = torch.rand(B, device=dev), torch.ones(B, device=dev)
+            for name, kw in (("plain", {}), ("top_k", {"top_k": torch.full((B,), 50, dtype=torch.int32, device=dev)}),
+                             ("top_p", {"top_p": torch.full((B,), 0.9, device=dev)})):
+                ms = timeit(lambda i=0: ops.sample_uniform(lg, u, tt, **kw))
+                report(f"sample_uniform_{name}", ms, None, B * V * 2, {"rows": B})
+        del kv, lg
+
     if not args.only or "moe" in args.only:
         # Qwen3-30B-A3B expert FFN at EP=8: 16 local experts, 128 tokens x top-8, H 2048, I 768
         from bloom_b200.models.config import preset

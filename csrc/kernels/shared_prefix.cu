@@ -1031,7 +1031,14 @@ void run(const CUtensorMap& tm, const Args& a, int items, int tile_rows, int pre
   // the suffix kernel starts as early, but its wait for the prefix kernel does not end while its CTAs load: 119 us for
   // 256 sequences behind 8,192 tokens, 108 this way; 120 and 103 for 16 groups of 8 that verify four tokens.  With one
   // row tile the prefix is short, and the third launch costs more than it gives: 28 us and 30.)
-  const c10::cuda::CUDAStream side = at::cuda::getStreamFromPool(false, stream.device_index());
+  // A pool's stream may be the caller's own, or one that another thread captures into: then the next, or none.
+  c10::cuda::CUDAStream side = stream;
+  for (int i = 0; i < 32 && side == stream; ++i) {
+    const c10::cuda::CUDAStream s = at::cuda::getStreamFromPool(false, stream.device_index());
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    C10_CUDA_CHECK(cudaStreamIsCapturing(s, &st));
+    if (st == cudaStreamCaptureStatusNone) side = s;
+  }
   at::cuda::CUDAEvent fork, join;
   fork.record(stream);
   fork.block(side);

@@ -217,6 +217,50 @@ def test_graph_replay_and_two_streams():
     c.check(outs[2])
 
 
+def test_large_groups_in_graphs_and_on_many_streams():
+    """Prefix and suffixes run on two streams there: calls from 40 streams of the pool, captured and eager."""
+    b = Batch((32, 8, 128), [70, 2], [400, 130], [1, 20, 90], seed=4)
+    want = b.run()
+    b.check(want)
+    outs = [torch.empty_like(b.q) for _ in range(40)]
+    torch.cuda.synchronize()
+    for out in outs:
+        with torch.cuda.stream(torch.cuda.Stream()):
+            b.run(out)
+    torch.cuda.synchronize()
+    for out in outs:
+        assert torch.equal(out, want)
+    graphs = []
+    for out in outs[:2]:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            b.run(out)
+            b.run(out)
+    outs[0].fill_(3), outs[1].fill_(3)
+    torch.cuda.synchronize()
+    s, t = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(5):
+        with torch.cuda.stream(s):
+            graphs[0].replay()
+        with torch.cuda.stream(t):
+            graphs[1].replay()
+        b.run(outs[2])
+    torch.cuda.synchronize()
+    for out in outs[:3]:
+        assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("members", [3, 9, 20, 70])
+def test_queries_before_the_first_token(members):
+    """Verify rows of sequences shorter than q_len: positions before the first token see nothing and give zeros."""
+    b = Batch((32, 8, 128), [members], [40], [4, 30], q_len=4)
+    lens = b.lens.clone()
+    lens[::2] = 2
+    out = b.run(lens=lens)
+    b.check(out, lens=lens)
+    assert bool((out.view(members, 4, 32, 128)[::2, :2] == 0).all())
+
+
 # ---------------------------------------------------------------- pages
 def page_state(kind, lens, seed=0, spare=6, layers=2):
     g = torch.Generator().manual_seed(seed)
