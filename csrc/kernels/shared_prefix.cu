@@ -21,12 +21,15 @@
 // zeroed in shared memory.  A block id outside the cache sets kStatusBadArgument and page 0 is read instead.
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/CUDAEvent.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cooperative_groups.h>
 #include <torch/extension.h>
 
 #include <algorithm>
 #include <atomic>
+#include <mutex>
+#include <vector>
 
 #include "bloom/common.cuh"
 #include "bloom/ops_share.h"
@@ -1019,6 +1022,59 @@ void run_suffix(const CUtensorMap& tm, const Args& a, int splits, int first_part
   else launch_suffix<D, 4, kMerge>(tm, a, splits, first_part, dependent, sms, stream);
 }
 
+// Streams of one device for the suffixes of groups of many rows.  They are this file's own: PyTorch hands its pool's
+// streams to everybody, and a stream that is joined to a capture belongs to it until the capture ends, with whatever
+// its other users launch on it meanwhile.  The mutex is held from the choice of a stream until the caller's stream has
+// waited for it, so no other thread brings it into a capture in between.
+struct SideStreams {
+  static constexpr size_t kMost = 32;  // captures under way may need more
+  struct Side {
+    cudaStream_t stream, caller;
+  };
+  std::mutex mutex;
+  std::vector<Side> all;
+  size_t next = 0;
+
+  // For a capturing caller a stream of its capture (it is there from an earlier call) or a free one, otherwise a free
+  // one; each caller's own where it has one, so that callers do not wait for one another.
+  c10::cuda::CUDAStream take(const c10::cuda::CUDAStream& caller) {
+    auto info = [](cudaStream_t s, unsigned long long& id) {
+      cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+      id = 0;
+      C10_CUDA_CHECK(cudaStreamGetCaptureInfo(s, &st, &id));
+      return st;
+    };
+    unsigned long long capture = 0, id = 0;
+    const bool capturing = info(caller.stream(), capture) == cudaStreamCaptureStatusActive;
+    size_t found = all.size();
+    for (size_t k = 0; k < all.size(); ++k) {
+      const size_t i = (next + k) % all.size();
+      const cudaStreamCaptureStatus st = info(all[i].stream, id);
+      const bool fits = st == cudaStreamCaptureStatusNone ||
+                        (capturing && st == cudaStreamCaptureStatusActive && id == capture);
+      if (!fits) continue;
+      if (all[i].caller == caller.stream()) return c10::cuda::getStreamFromExternal(all[i].stream, caller.device_index());
+      if (found == all.size() && st == cudaStreamCaptureStatusNone) found = i;
+    }
+    if (all.size() < kMost || found == all.size()) {
+      // not an operation of the capture, but one that its mode may forbid
+      const c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+      cudaStream_t s = nullptr;
+      C10_CUDA_CHECK(cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking));
+      found = all.size();
+      all.push_back({s, nullptr});
+    }
+    next = (found + 1) % all.size();
+    all[found].caller = caller.stream();
+    return c10::cuda::getStreamFromExternal(all[found].stream, caller.device_index());
+  }
+};
+// Never destroyed: streams outlive the CUDA context's end at exit.
+SideStreams& side_streams(int device) {
+  static SideStreams* const per_device = new SideStreams[64];
+  return per_device[device];
+}
+
 template <int D>
 void run(const CUtensorMap& tm, const Args& a, int items, int tile_rows, int prefix_parts, int suffix_splits, int sms,
          c10::cuda::CUDAStream stream) {
@@ -1036,14 +1092,9 @@ void run(const CUtensorMap& tm, const Args& a, int items, int tile_rows, int pre
   // the suffix kernel starts as early, but its wait for the prefix kernel does not end while its CTAs load: 119 us for
   // 256 sequences behind 8,192 tokens, 108 this way; 120 and 103 for 16 groups of 8 that verify four tokens.  With one
   // row tile the prefix is short, and the third launch costs more than it gives: 28 us and 30.)
-  // A pool's stream may be the caller's own, or one that another thread captures into: then the next, or none.
-  c10::cuda::CUDAStream side = stream;
-  for (int i = 0; i < 32 && side == stream; ++i) {
-    const c10::cuda::CUDAStream s = at::cuda::getStreamFromPool(false, stream.device_index());
-    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-    C10_CUDA_CHECK(cudaStreamIsCapturing(s, &st));
-    if (st == cudaStreamCaptureStatusNone) side = s;
-  }
+  SideStreams& streams = side_streams(stream.device_index());
+  const std::lock_guard<std::mutex> lock(streams.mutex);
+  const c10::cuda::CUDAStream side = streams.take(stream);
   at::cuda::CUDAEvent fork, join;
   fork.record(stream);
   fork.block(side);

@@ -576,3 +576,91 @@ def test_many_completions_of_one_prompt():
         step()
     ops.kv_free(table, lens, i32(list(range(10))), count)
     assert int(count.abs().sum()) == 0 and int(lens.sum()) == 0
+
+
+# ---------------------------------------------------------------- the side stream of large groups
+def large_batch(seed=6):
+    """A group of more than 128 query rows per KV head: prefix and suffixes run side by side on two streams."""
+    b = Batch((32, 8, 128), [70, 2], [400, 130], [1, 20, 90], seed=seed)
+    assert b.plan.tile_rows == 256
+    return b
+
+
+def test_every_large_group_call_of_a_capture_runs_side_by_side(tmp_path):
+    """In a graph of 40 calls (a model's layers) of three kernels each, the longest chain is two kernels a call: prefix
+    and suffixes do not wait for one another."""
+    import re
+
+    b = large_batch()
+    out = torch.empty_like(b.q)
+    b.run(out)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(g):
+        for _ in range(40):
+            b.run(out)
+    path = tmp_path / "graph.dot"
+    g.debug_dump(str(path))
+    edges = set(re.findall(r'"([^"]+)"\s*->\s*"([^"]+)"', path.read_text()))
+    follow, waits = {}, {}
+    for a, z in edges:
+        follow.setdefault(a, []).append(z)
+        waits[z] = waits.get(z, 0) + 1
+    nodes = {n for e in edges for n in e}
+    depth = dict.fromkeys(nodes, 1)
+    ready = [n for n in nodes if n not in waits]
+    while ready:
+        n = ready.pop()
+        for z in follow.get(n, []):
+            depth[z] = max(depth[z], depth[n] + 1)
+            waits[z] -= 1
+            if waits[z] == 0:
+                ready.append(z)
+    assert len(nodes) == 120 and max(depth.values()) == 80
+
+
+def test_capture_of_large_groups_takes_no_stream_of_others():
+    """While a capture holds 40 large-group calls, work of another thread on any of PyTorch's streams runs at once and
+    is not recorded, an eager call of another thread included."""
+    import threading
+
+    b = large_batch()
+    want = b.run()
+    out, other = torch.empty_like(b.q), torch.full_like(b.q, 5.0)
+    streams = [torch.cuda.Stream() for _ in range(32)]
+    x = torch.zeros(32, device="cuda")
+    x[0].add_(0)
+    torch.cuda.synchronize()
+    failed, skipped = [], []
+
+    def work(capturing):
+        try:
+            for i, s in enumerate(streams):
+                if s.cuda_stream == capturing:
+                    skipped.append(i)
+                    continue
+                with torch.cuda.stream(s):
+                    x[i].add_(1)
+                    if i == 3 or (i == 4 and 3 in skipped):
+                        b.run(other)
+        except Exception as e:  # noqa: BLE001  (shown by the assertion below)
+            failed.append(e)
+
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, capture_error_mode="thread_local"):
+        for _ in range(40):
+            b.run(out)
+        t = threading.Thread(target=work, args=(torch.cuda.current_stream().cuda_stream,))
+        t.start()
+        t.join()
+        b.run(out)
+    torch.cuda.synchronize()
+    assert not failed, failed
+    ones = torch.ones(32, device="cuda")
+    ones[skipped] = 0
+    assert torch.equal(x, ones) and torch.equal(other, want)
+    out.fill_(3)
+    other.fill_(4)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and torch.equal(x, ones) and bool((other == 4).all())
