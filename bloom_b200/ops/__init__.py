@@ -654,10 +654,11 @@ def kv_fork(kv_cache, block_table, seq_lens, parents, fresh, ref):
     kv_cache [L, NB, ...] of any type, contiguous; block_table int32 [S, W]; seq_lens int32 [S]; parents, fresh
     int32 [C]; ref int32 [NB], the number of rows that hold each page, raised for every page taken.  Returns
     (table int32 [C, W], lens int32 [C]), entries behind the last page 0.  parents[c] < 0 gives an empty row;
-    fresh[c] is not looked at where the parent's last page is full.  An id out of range, or a fresh page that is
-    not free, sets status bit 8 (`check_status`); such a call's results are not to be used."""
+    fresh[c] is not looked at where the parent's last page is full.  A child with an id out of range, or whose fresh
+    page is not free (two children may not share one), sets status bit 8 (`check_status`) and gets an empty row; nothing
+    is copied or counted for it, and the other children are made."""
     r = _C().kv_fork(kv_cache, block_table, seq_lens, parents, fresh, ref)
-    _count()
+    _count(2 if parents.shape[0] else 0)
     return r
 
 

@@ -5,13 +5,15 @@
 // block-table rows that hold a page (0: free).
 //
 //   fork     row c of the new table takes the parent's pages; ref += 1 on each; a last page that is not full is
-//            copied to fresh[c], because parent and child will write different tokens into it
+//            copied to fresh[c], because parent and child will write different tokens into it.  A child whose ids are
+//            out of range or whose fresh page is held gets an empty row
 //   free     ref -= 1 on a row's pages, and its length becomes 0 (a second free of the row is a no-op)
 //   compact  U = pages held; the i-th held page at or above U moves to the i-th free page below U (the two sets are
 //            disjoint and equally large, so all copies may run at once); tables and ref follow
 //
 // All three are bound by the bytes of the pages they copy (each read once and written once), and at small sizes by
-// launches: fork and free are one launch, compact is two (a one-CTA plan over a bitmap of ref, then the copies).
+// launches: free is one launch, fork two (rows and claims, then the copies) and compact two (a one-CTA plan over a bitmap of
+// ref, then the copies).
 // Copies run in chunks of 16 or 32 KB per CTA, all loads of a chunk in flight before its first store: 8 CTAs per SM
 // keep 128 KB or more in flight, which covers the bandwidth-latency product (44 GB/s per SM x ~2 us).
 // Measured: a pool of 18,000 pages compacts at 6.5 TB/s (read + write) after a plan of 8 to 11 us; a fork of 4 children takes
@@ -47,13 +49,15 @@ __device__ __forceinline__ void bad(int* status) { atomicOr(status, kStatusBadAr
 
 // One chunk of one page: bytes [off, off + kChunk<kVec>) below `bytes` (a multiple of 16).
 template <int kVec>
-__device__ __forceinline__ void copy_chunk(const uint8_t* src, uint8_t* dst, long off, long bytes) {
-  uint4 v[kVec];
+__device__ __forceinline__ void load_chunk(const uint8_t* src, long off, long bytes, uint4 (&v)[kVec]) {
 #pragma unroll
   for (int i = 0; i < kVec; ++i) {
     const long o = off + (long)(i * kThreads + threadIdx.x) * 16;
     if (o < bytes) v[i] = __ldg(reinterpret_cast<const uint4*>(src + o));
   }
+}
+template <int kVec>
+__device__ __forceinline__ void store_chunk(uint8_t* dst, long off, long bytes, const uint4 (&v)[kVec]) {
 #pragma unroll
   for (int i = 0; i < kVec; ++i) {
     const long o = off + (long)(i * kThreads + threadIdx.x) * 16;
@@ -77,58 +81,60 @@ struct ForkArgs {
   int* status;
 };
 
-// grid (1 + layers * chunks, children): CTA 0 of a child writes its row, the others copy.
-__global__ void __launch_bounds__(kThreads) fork_kernel(const ForkArgs a) {
-  const int c = blockIdx.y;
+// Fork, first kernel: one CTA per child checks it, claims its fresh page and writes its row.  A child is made whole or
+// not at all, and the claim (0 -> 1 on the count of a page that is free) comes before any byte of the page is written:
+// a page that somebody holds, or that another child has claimed, is left as it is.
+__global__ void __launch_bounds__(kThreads) fork_rows_kernel(const ForkArgs a) {
+  griddep_launch_dependents();
+  const int c = blockIdx.x;
   const int p = a.parents[c], f = a.fresh[c];
-  const bool writer = blockIdx.x == 0;
   int len = 0;
-  bool ok = p >= 0;
-  if (ok && p >= a.S) {
-    ok = false;
-    if (writer && threadIdx.x == 0) bad(a.status);
-  }
+  bool ok = p >= 0 && p < a.S;
   if (ok) {
     len = a.lens[p];
-    // the fresh page is needed (and looked at) only where the last page is not full
-    if (len < 0 || len > a.W * kPage || (len % kPage != 0 && (f < 0 || f >= a.NB))) {
-      ok = false;
-      if (writer && threadIdx.x == 0) bad(a.status);
-    }
+    ok = len >= 0 && len <= a.W * kPage;
   }
-  if (!ok) len = 0;
-  const int full = len / kPage;
+  const int n = ok ? (len + kPage - 1) / kPage : 0, full = len / kPage;
   const int* row = a.table + (long)(ok ? p : 0) * a.table_stride;
-  if (writer) {
-    for (int j = threadIdx.x; j < a.W; j += kThreads) {
-      int page = 0;
-      if (j < full) {
-        page = row[j];
-        if (page >= 0 && page < a.NB) {
-          atomicAdd(a.ref + page, 1);
-        } else {
-          page = 0;
-          bad(a.status);
-        }
-      } else if (j == full && len % kPage != 0) {
-        page = f;
-        if (atomicAdd(a.ref + f, 1) != 0) bad(a.status);  // not free, or given to two children
-      }
-      a.out_table[(long)c * a.W + j] = page;
+  for (int j = threadIdx.x; j < n; j += kThreads) ok = ok && row[j] >= 0 && row[j] < a.NB;
+  // the fresh page is needed (and looked at) only where the last page is not full
+  if (ok && n > full && threadIdx.x == 0) ok = f >= 0 && f < a.NB && row[full] != f;
+  ok = __syncthreads_and(ok);
+  if (ok && n > full && threadIdx.x == 0) ok = atomicCAS(a.ref + f, 0, 1) == 0;
+  ok = __syncthreads_and(ok);
+  for (int j = threadIdx.x; j < a.W; j += kThreads) {
+    int page = 0;
+    if (ok && j < full) {
+      page = row[j];
+      atomicAdd(a.ref + page, 1);
+    } else if (ok && j < n) {
+      page = f;
     }
-    if (threadIdx.x == 0) a.out_lens[c] = len;
-    return;
+    a.out_table[(long)c * a.W + j] = page;
   }
-  if (len % kPage == 0) return;
-  const int src = row[full];
-  if (src < 0 || src >= a.NB || src == f) {
-    if (threadIdx.x == 0) bad(a.status);
-    return;
+  if (threadIdx.x == 0) {
+    a.out_lens[c] = ok ? len : 0;
+    if (!ok && p >= 0) bad(a.status);
   }
-  const int item = blockIdx.x - 1;
-  const long layer = (long)(item / a.chunks) * a.layer_bytes;
-  copy_chunk<kForkVec>(a.cache + layer + src * a.page_bytes, a.cache + layer + f * a.page_bytes,
-                       (long)(item % a.chunks) * kChunk<kForkVec>, a.page_bytes);
+}
+
+// Second kernel, grid (layers * chunks, children): copies the unfinished page of each child that was made.  A dependent
+// of the first: by the time that is done, a chunk of the source (a held page, which no child can have claimed) is in
+// registers, and all that follows the wait is a look at the child's length and the stores.
+__global__ void __launch_bounds__(kThreads) fork_copy_kernel(const ForkArgs a) {
+  const int c = blockIdx.y;
+  const int p = a.parents[c], f = a.fresh[c];
+  const int len = p >= 0 && p < a.S ? a.lens[p] : 0;
+  const bool partial = len > 0 && len <= a.W * kPage && len % kPage != 0 && f >= 0 && f < a.NB;
+  const int src = partial ? a.table[(long)p * a.table_stride + len / kPage] : -1;
+  const bool there = src >= 0 && src < a.NB && src != f;
+  const long layer = (long)(blockIdx.x / a.chunks) * a.layer_bytes;
+  const long off = (long)(blockIdx.x % a.chunks) * kChunk<kForkVec>;
+  uint4 v[kForkVec];
+  if (there) load_chunk<kForkVec>(a.cache + layer + src * a.page_bytes, off, a.page_bytes, v);
+  griddep_wait();
+  if (there && *const_cast<const volatile int*>(a.out_lens + c) == len)  // 0 where the child was refused
+    store_chunk<kForkVec>(a.cache + layer + f * a.page_bytes, off, a.page_bytes, v);
 }
 
 struct FreeArgs {
@@ -319,8 +325,9 @@ __global__ void __launch_bounds__(kThreads) move_kernel(const CompactArgs a) {
     const int l = int(ml % a.L);
     const int m = int(ml / a.L);
     const long layer = (long)l * a.layer_bytes;
-    copy_chunk<kMoveVec>(a.cache + layer + a.src[m] * a.page_bytes, a.cache + layer + a.dst[m] * a.page_bytes,
-                         (long)chunk * kChunk<kMoveVec>, a.page_bytes);
+    uint4 v[kMoveVec];
+    load_chunk<kMoveVec>(a.cache + layer + a.src[m] * a.page_bytes, (long)chunk * kChunk<kMoveVec>, a.page_bytes, v);
+    store_chunk<kMoveVec>(a.cache + layer + a.dst[m] * a.page_bytes, (long)chunk * kChunk<kMoveVec>, a.page_bytes, v);
   }
 }
 
@@ -387,9 +394,19 @@ std::tuple<torch::Tensor, torch::Tensor> kv_fork(torch::Tensor& kv_cache, const 
   a.out_table = table.data_ptr<int>();
   a.out_lens = lens.data_ptr<int>();
   a.status = status_word(kv_cache.get_device());
-  const dim3 grid(unsigned(1 + kv_cache.size(0) * a.chunks), unsigned(C));
-  fork_kernel<<<grid, kThreads, 0, at::cuda::getCurrentCUDAStream()>>>(a);
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  fork_rows_kernel<<<unsigned(C), kThreads, 0, stream>>>(a);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(kv_cache.size(0) * a.chunks), unsigned(C));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fork_copy_kernel, a));
   return {table, lens};
 }
 

@@ -664,3 +664,51 @@ def test_capture_of_large_groups_takes_no_stream_of_others():
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want) and torch.equal(x, ones) and bool((other == 4).all())
+
+
+# ---------------------------------------------------------------- children that are refused
+@pytest.mark.parametrize("kw", ["parent", "fresh", "taken", "taken by many", "source", "twice", "page", "last page",
+                                "length"])
+def test_kv_fork_refuses_a_child_and_leaves_the_rest(kw):
+    """A child that cannot be made gets an empty row, and nothing is copied, counted or changed for it; the other children
+    are made."""
+    cache, table, n, count, free = page_state("int8", [20, 40, 5])
+    count[table[2, 0].long()] = 3
+    parents, fresh = i32([0, 1, 2]), i32(free[:3])
+    if kw == "parent":
+        parents[1] = 3
+    elif kw == "fresh":
+        fresh[1] = cache.shape[1]
+    elif kw == "taken":
+        fresh[1] = table[0, 0]
+    elif kw == "taken by many":
+        fresh[1] = table[2, 0]
+    elif kw == "source":
+        fresh[1] = table[1, 2]
+    elif kw == "twice":
+        fresh[1] = fresh[0]
+    elif kw == "page":
+        table[1, 1] = -4
+    elif kw == "last page":
+        table[1, 2] = cache.shape[1]
+    else:
+        n[1] = 16 * table.shape[1] + 1
+    args = (cache, table, n, parents, fresh, count)
+    want = [t.clone() for t in args]
+    made = [0, 2]
+    if kw == "twice":  # one of the two is made
+        want_rows = [{0, 2}, {1, 2}]
+    else:
+        want_rows = [set(made)]
+    t, lens = ops.kv_fork(*args)
+    assert took_bits() == BAD
+    got = {c for c in range(3) if int(lens[c]) > 0}
+    assert got in want_rows
+    wp = want[3].clone()
+    for c in range(3):
+        if c not in got:
+            wp[c] = -1
+    wt, wl = ref.kv_fork(want[0], want[1], want[2], wp, want[4], want[5])
+    assert torch.equal(t, wt) and torch.equal(lens, wl)
+    assert torch.equal(cache, want[0]) and torch.equal(count, want[5])
+    assert torch.equal(table, want[1]) and torch.equal(n, want[2])
