@@ -115,7 +115,7 @@ __device__ __forceinline__ float value_of(unsigned key) {
 }
 
 struct Row {
-  float mx, bins;      // bins per unit of l
+  float step, top, bins;  // a power of two, the maximum times it, bins per unit of l times it
   float low;           // values below it have no mass
   double mxd, c;       // the maximum, 512 / (t ln 2)
 };
@@ -140,9 +140,10 @@ __device__ __forceinline__ u64 mass_if(bool keep, float v, const Row& r, const d
   const u64 m = mass_of(v, r, tab);
   return keep ? m : 0;
 }
-// First-level bin of l >= low: monotone in l, because every rounding in it is.
+// First-level bin of l >= low: monotone in l, because every rounding in it is.  The distance (max - l) step is rounded
+// once; the step is 1 unless the distance or the bins per unit could leave fp32's range.
 __device__ __forceinline__ int bin_of(float l, const Row& r) {
-  return min(static_cast<int>((r.mx - l) * r.bins), kBins - 1);
+  return min(static_cast<int>(fmaf(-l, r.step, r.top) * r.bins), kBins - 1);
 }
 
 // 8 consecutive tokens from the slice.
@@ -557,11 +558,15 @@ __global__ void __launch_bounds__(kThreads, 2) draw_kernel(const Args a) {
   }
   __syncthreads();
   Row r;
-  r.mx = best;
   const double td = static_cast<double>(t);
+  // max - l may be twice the largest float, which matters where t is as large; 1 / t overflows below 2^-128, and
+  // distances of t / 32 are subnormal (0 here) below 2^-121.  With such a t and a maximum of 1 or more, all of l >= low
+  // equal the maximum.
+  r.step = t > 0x1p64f ? 0.25f : t < 0x1p-100f && fabsf(best) < 1.f ? 0x1p100f : 1.f;
+  r.top = best * r.step;
   r.c = 738.65986093514926 / td;  // 512 / ln 2
   r.mxd = static_cast<double>(best);
-  r.bins = static_cast<float>(kBinsPerT / td);
+  r.bins = static_cast<float>(kBinsPerT / (td * static_cast<double>(r.step)));
   r.low = fmaxf(static_cast<float>(static_cast<double>(best) - kRange * td), -FLT_MAX);
   const bool need_k = k > 0 && k < a.V, need_p = p > 0.f && p < 1.f;
   Cut cut{r.low, 0x7fffffff};

@@ -712,3 +712,25 @@ def test_kv_fork_refuses_a_child_and_leaves_the_rest(kw):
     assert torch.equal(t, wt) and torch.equal(lens, wl)
     assert torch.equal(cache, want[0]) and torch.equal(count, want[5])
     assert torch.equal(table, want[1]) and torch.equal(n, want[2])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("t", [1e37, 1e38, 3e38, 2e-38, 8e-38, 1e-36])
+def test_sample_uniform_largest_and_smallest_temperatures(t, dtype):
+    """Distances to the maximum, in units of the temperature, whose parts leave fp32's range: the cut of top-p is
+    right all the same."""
+    g = torch.Generator(device="cuda").manual_seed(11)
+    if t > 1:
+        logits = (torch.rand(6, 3001, generator=g, device="cuda") * 2 - 1) * 3e38
+        logits[:, 7] = 3.2e38
+        logits[3] = torch.where(logits[3] > 0, 3e38, -3e38)
+    else:
+        logits = torch.rand(6, 3001, generator=g, device="cuda") * 12 * t + 2 * t
+        logits[3] = torch.where(logits[3] > 8 * t, 10 * t, 6 * t)
+    logits = logits.to(dtype)
+    u = torch.rand(6, 20, generator=g, device="cuda")
+    check_draw(logits, u, [t])
+    check_draw(logits, u, [t], top_k=[1, 40, 400, 1000, 2999, 0])
+    for p in (0.2, 0.5, 0.9, 0.99):
+        check_draw(logits, u, [t], top_p=[p])
+        check_draw(logits, u, [t], top_p=[p], top_k=[700])
