@@ -833,9 +833,11 @@ def sample_uniform(logits, u, temperature, top_k=None, top_p=None, min_p=None, o
     Weights exp((l - max) / temperature); top_k (int32 [B]) keeps the k largest, ties to the lowest index; top_p
     (f32 [B]) then keeps, in falling order, every token with less than top_p of the remaining mass ahead of it; min_p
     (f32 [B]) drops weights below min_p times the largest.  The token is the first kept one, in vocabulary order,
-    whose running sum exceeds u times the kept mass.  temperature <= 0: the largest logit (lowest index).  top_k <= 0,
-    top_p outside (0, 1), min_p <= 0 or an absent tensor: off.  NaN logits count as -inf; a row with nothing to draw
-    from gives -1.  u is taken into [0, 1].  Sums are exact integers: equal inputs give equal tokens."""
+    whose running sum exceeds u times the kept mass.  temperature <= 0 or NaN: the largest logit (lowest index).
+    top_k <= 0, top_p outside (0, 1), min_p <= 0, NaN in either or an absent tensor: off.  NaN logits count as -inf; a
+    row with nothing to draw from gives -1.  u is taken into [0, 1], NaN as 0.  Sums are exact integers: equal inputs
+    give equal tokens.  Weights below 2^-46 of the largest count as 0 (such tokens are never drawn), and subnormal logits
+    and temperatures as 0."""
     if out is None:
         out = torch.empty(u.shape, dtype=torch.int32, device=u.device)
     _C().sample_uniform(logits, u, temperature, top_k, top_p, min_p, out)

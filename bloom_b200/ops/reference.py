@@ -291,7 +291,7 @@ def sample_uniform(logits, u, temperature, top_k=None, top_p=None, min_p=None):
             cum = torch.cumsum(w[order], 0)
             ahead = torch.cat([torch.zeros(1, dtype=torch.float64), cum[:-1]])
             order = order[ahead < p * cum[-1]]
-        floor = 0.0 if min_p is None else min(1.0, float(min_p[b]))
+        floor = 0.0 if min_p is None or math.isnan(min_p[b]) else min(1.0, float(min_p[b]))
         order = order[(w[order] >= floor) & (w[order] > 0)]
         ids = order.sort()[0]
         cum = torch.cumsum(w[ids], 0)

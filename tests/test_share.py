@@ -170,3 +170,15 @@ def test_oracle_pages():
     assert used.tolist() == [3] and moved.tolist() == [-1, -1, 2, 0, -1, 1]
     assert t.tolist() == [[0, 2], [1, 0], [0, 0]] and count.tolist() == [1, 2, 1, 0, 0, 0]
     assert cache[0, :3, 0].tolist() == [3, 5, 1]
+
+
+def test_oracle_draw_with_nan_settings():
+    """NaN is in no range that a setting is on in: off, and a NaN temperature is greedy."""
+    nan = torch.tensor([float("nan")])
+    logits = torch.log(torch.tensor([[2.0, 4.0, 1.0, 1.0]]))
+    u = torch.tensor([[0.0, 0.4, 0.6, 0.8, 0.95]])
+    plain = ref.sample_uniform(logits, u, torch.ones(1)).tolist()
+    assert plain == [[0, 1, 1, 2, 3]]
+    assert ref.sample_uniform(logits, u, torch.ones(1), min_p=nan).tolist() == plain
+    assert ref.sample_uniform(logits, u, torch.ones(1), top_p=nan).tolist() == plain
+    assert ref.sample_uniform(logits, u, nan).tolist() == [[1] * 5]

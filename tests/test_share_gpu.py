@@ -734,3 +734,15 @@ def test_sample_uniform_largest_and_smallest_temperatures(t, dtype):
     for p in (0.2, 0.5, 0.9, 0.99):
         check_draw(logits, u, [t], top_p=[p])
         check_draw(logits, u, [t], top_p=[p], top_k=[700])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_sample_uniform_nan_settings(dtype):
+    nan = float("nan")
+    g = torch.Generator(device="cuda").manual_seed(13)
+    logits = (torch.randn(4, 3001, generator=g, device="cuda") * 2).to(dtype)
+    u = torch.rand(4, 9, generator=g, device="cuda")
+    plain = check_draw(logits, u, [0.8])
+    assert torch.equal(check_draw(logits, u, [0.8], top_p=[nan], min_p=[nan]), plain)
+    check_draw(logits, u, [0.8], top_k=[30], top_p=[0.7, nan, nan, 0.9], min_p=[nan, 0.1, nan, 0.2])
+    check_draw(logits, u, [nan], top_k=[30])
