@@ -634,7 +634,7 @@ def shared_prefix_attention(q, kv_cache, layer, block_table, seq_lens, out, *, p
     Same result as `paged_decode_attention` over the same tables: query position i of a sequence sees keys
     0 .. seq_len - q_len + i.  All members of a group must hold the same K / V for the group's prefix (in the same
     pages or in copies); it is read through the first member that still holds it.  seq_lens of 0 (padding, ended
-    members) give zeros.  Slots behind a sequence's end may hold anything.  Safe in CUDA graphs: the workspace
+    members) give zeros.  Slots behind a sequence's end may hold anything.  scale must be finite.  Safe in CUDA graphs: the workspace
     belongs to the call.  Only bf16 caches (an int8 cache is refused)."""
     if (q.dim() == 3 and (q.shape[1] != plan.num_q_heads or q.shape[2] != plan.head_dim)) or \
             (kv_cache.dim() == 6 and kv_cache.shape[3] != plan.num_kv_heads):

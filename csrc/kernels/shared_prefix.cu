@@ -28,6 +28,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <mutex>
 #include <vector>
 
@@ -1150,6 +1151,7 @@ void shared_prefix_attention(const torch::Tensor& q, const torch::Tensor& kv_cac
   const uint64_t rows = (uint64_t)kv_cache.size(1) * 2 * nkv * PAGE;
   SP_CHECK(rows < (1ull << 31), "kv_cache has too many rows per layer for 32-bit tile coordinates");
   SP_CHECK(nkv * q.size(1) * q_len <= 65535, "too many heads");
+  SP_CHECK(std::isfinite(float(scale * 1.4426950408889634)), "scale must be a finite number");
   SP_CHECK(q.is_cuda(), "tensors must be on a CUDA device");
   for (const torch::Tensor* t : {&kv_cache, &block_table, &seq_lens, &static_cast<const torch::Tensor&>(out), &items,
                                  &groups, &seqs})

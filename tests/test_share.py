@@ -182,3 +182,9 @@ def test_oracle_draw_with_nan_settings():
     assert ref.sample_uniform(logits, u, torch.ones(1), min_p=nan).tolist() == plain
     assert ref.sample_uniform(logits, u, torch.ones(1), top_p=nan).tolist() == plain
     assert ref.sample_uniform(logits, u, nan).tolist() == [[1] * 5]
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), float("-inf"), 3e38])
+def test_shared_prefix_attention_refuses_scales(scale):
+    with pytest.raises(RuntimeError, match="scale must be"):
+        ops.shared_prefix_attention(**shared_args(), scale=scale)
