@@ -1150,7 +1150,8 @@ void shared_prefix_attention(const torch::Tensor& q, const torch::Tensor& kv_cac
   SP_CHECK(suffix_splits == 1 || suffix_splits == 2 || suffix_splits == 4 || suffix_splits == 8, "suffix_splits must be 1, 2, 4 or 8");
   const uint64_t rows = (uint64_t)kv_cache.size(1) * 2 * nkv * PAGE;
   SP_CHECK(rows < (1ull << 31), "kv_cache has too many rows per layer for 32-bit tile coordinates");
-  SP_CHECK(nkv * q.size(1) * q_len <= 65535, "too many heads");
+  // the suffix grid's second dimension: KV heads x chunks of up to 32 query rows
+  SP_CHECK(nkv * ((q_len * (q.size(1) / nkv) + 31) / 32) <= 65535, "too many heads x query rows");
   SP_CHECK(std::isfinite(float(scale * 1.4426950408889634)), "scale must be a finite number");
   SP_CHECK(q.is_cuda(), "tensors must be on a CUDA device");
   for (const torch::Tensor* t : {&kv_cache, &block_table, &seq_lens, &static_cast<const torch::Tensor&>(out), &items,

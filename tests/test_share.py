@@ -188,3 +188,16 @@ def test_oracle_draw_with_nan_settings():
 def test_shared_prefix_attention_refuses_scales(scale):
     with pytest.raises(RuntimeError, match="scale must be"):
         ops.shared_prefix_attention(**shared_args(), scale=scale)
+
+
+@pytest.mark.parametrize("q_len,msg", [(128, "CUDA device"), (1 << 14, "CUDA device"), (1 << 16, "too many heads")])
+def test_shared_prefix_attention_query_rows(q_len, msg):
+    """As many query rows as the grid holds: KV heads x chunks of 32 rows up to 65,535."""
+    nq, nkv = 64, 32
+    q = torch.zeros(1, nq, 64, dtype=torch.bfloat16).expand(q_len, nq, 64)
+    a = shared_args(q=q, out=torch.empty(q_len, nq, 64, dtype=torch.bfloat16), seq_lens=i32(20),
+                    kv_cache=torch.zeros(1, 6, 2, nkv, 16, 64, dtype=torch.bfloat16),
+                    block_table=torch.zeros(1, 3, dtype=torch.int32),
+                    plan=ops.shared_prefix_plan([1], [16], num_q_heads=nq, num_kv_heads=nkv, head_dim=64, q_len=q_len))
+    with pytest.raises(RuntimeError, match=msg):
+        ops.shared_prefix_attention(**a, scale=1.0)

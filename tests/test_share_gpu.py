@@ -746,3 +746,10 @@ def test_sample_uniform_nan_settings(dtype):
     assert torch.equal(check_draw(logits, u, [0.8], top_p=[nan], min_p=[nan]), plain)
     check_draw(logits, u, [0.8], top_k=[30], top_p=[0.7, nan, nan, 0.9], min_p=[nan, 0.1, nan, 0.2])
     check_draw(logits, u, [nan], top_k=[30])
+
+
+@pytest.mark.parametrize("heads,q_len", [((64, 8, 128), 130), ((8, 8, 64), 1100), ((32, 8, 128), 300)])
+def test_many_query_rows(heads, q_len):
+    """Prompts behind a shared prefix: query positions by the hundred for each sequence."""
+    b = Batch(heads, [2, 1], [100, 33], [q_len, q_len + 7], q_len=q_len)
+    b.check(b.run())
