@@ -633,9 +633,14 @@ def shared_prefix_attention(q, kv_cache, layer, block_table, seq_lens, out, *, p
 
     Same result as `paged_decode_attention` over the same tables: query position i of a sequence sees keys
     0 .. seq_len - q_len + i.  All members of a group must hold the same K / V for the group's prefix (in the same
-    pages or in copies); it is read through the first member that still holds it.  seq_lens of 0 (padding, ended
-    members) give zeros.  Slots behind a sequence's end may hold anything.  scale must be finite.  Safe in CUDA graphs: the workspace
-    belongs to the call.  Only bf16 caches (an int8 cache is refused)."""
+    pages or in copies); it is read through the first member that holds the most of it.  seq_lens of 0 (padding, ended
+    members) give zeros.  Slots behind a sequence's end may hold anything; K / V that some rows of a group see and
+    others do not (later verify positions, a prefix that goes on behind a shorter member's end) must be finite.  scale
+    must be finite.  Only bf16 caches (an int8 cache is refused).
+
+    Safe in CUDA graphs, once `ops.status()` has been called outside of a capture: the workspace belongs to the call.
+    Where a group has more than 128 query rows per KV head, a stream of the library's own runs beside the caller's; the
+    caller's waits for it.  A block id out of range sets status bit 8 and page 0 is read instead."""
     if (q.dim() == 3 and (q.shape[1] != plan.num_q_heads or q.shape[2] != plan.head_dim)) or \
             (kv_cache.dim() == 6 and kv_cache.shape[3] != plan.num_kv_heads):
         raise ValueError("shared_prefix_attention: the plan was made for other heads")

@@ -753,3 +753,54 @@ def test_many_query_rows(heads, q_len):
     """Prompts behind a shared prefix: query positions by the hundred for each sequence."""
     b = Batch(heads, [2, 1], [100, 33], [q_len, q_len + 7], q_len=q_len)
     b.check(b.run())
+
+
+# ---------------------------------------------------------------- ids that are not followed
+@pytest.mark.parametrize("members", [3, 20, 70])
+@pytest.mark.parametrize("where", ["own", "prefix"])
+@pytest.mark.parametrize("below", [False, True])
+def test_bad_ids_read_page_0(members, where, below):
+    """The cache handed over is the middle of a larger one; ids that land in the rest of it are not followed: the
+    result is that of page 0 in their place."""
+    b = Batch((32, 8, 128), [members], [64], [20])
+    front = torch.nan_to_num(b.cache)
+    NB = front.shape[1]
+    big = torch.full((1, 3 * NB, *front.shape[2:]), 50.0, dtype=front.dtype, device="cuda")
+    big[:, NB:2 * NB] = front
+    b.cache = big[:, NB:2 * NB]
+    assert b.cache.is_contiguous()
+    bad = -2 if below else NB + 3
+    clean = b.table.clone()
+    if where == "own":
+        b.table[1, 5] = bad
+        clean[1, 5] = 0
+    else:  # the prefix is read through the first member's row
+        b.table[0, 2] = bad
+        clean[:, 2] = 0
+    out = b.run()
+    assert took_bits() == BAD
+    b.table = clean
+    b.check(out)
+
+
+@pytest.mark.parametrize("bad", [-1, 10**6])
+def test_kv_free_and_compact_pass_over_bad_ids(bad):
+    cache, table, n, count, free = page_state("int8", [40, 20, 100], spare=9)
+    want = [t.clone() for t in (cache, table, n, count)]
+    table[0, 1] = bad
+    keep = int(want[1][0, 1])  # the page that the bad id stands in place of: never given back
+    ops.kv_free(table, n, i32([0]), count)
+    assert took_bits() == BAD
+    want[3][want[1][0, [0, 2]].long()] -= 1
+    want[2][0] = 0
+    want[1][0, 1] = bad
+    assert int(count[keep]) == 1 and torch.equal(count, want[3]) and torch.equal(n, want[2])
+    table[1, 0] = bad
+    want[1][1, 0] = table[2, 0]  # for the oracle: any held page
+    moved, used = ref.kv_compact(*want)
+    want[1][1, 0] = bad
+    got = ops.kv_compact(cache, table, n, count)
+    assert took_bits() == BAD
+    assert torch.equal(got[0], moved) and torch.equal(got[1], used)
+    for a, w in zip((cache, table, n, count), want):
+        assert torch.equal(a, w)
