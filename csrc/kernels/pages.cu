@@ -324,10 +324,13 @@ __global__ void __launch_bounds__(kThreads) move_kernel(const CompactArgs a) {
     const long ml = it / a.chunks;
     const int l = int(ml % a.L);
     const int m = int(ml / a.L);
-    const long layer = (long)l * a.layer_bytes;
+    const long layer = (long)l * a.layer_bytes, off = (long)chunk * kChunk<kMoveVec>;
+    // both ids before the loads: the target's would otherwise be fetched after them
+    const uint8_t* from = a.cache + layer + a.src[m] * a.page_bytes;
+    uint8_t* to = a.cache + layer + a.dst[m] * a.page_bytes;
     uint4 v[kMoveVec];
-    load_chunk<kMoveVec>(a.cache + layer + a.src[m] * a.page_bytes, (long)chunk * kChunk<kMoveVec>, a.page_bytes, v);
-    store_chunk<kMoveVec>(a.cache + layer + a.dst[m] * a.page_bytes, (long)chunk * kChunk<kMoveVec>, a.page_bytes, v);
+    load_chunk<kMoveVec>(from, off, a.page_bytes, v);
+    store_chunk<kMoveVec>(to, off, a.page_bytes, v);
   }
 }
 
