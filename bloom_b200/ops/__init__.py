@@ -663,7 +663,7 @@ def kv_fork(kv_cache, block_table, seq_lens, parents, fresh, ref):
     page is not free (two children may not share one), sets status bit 8 (`check_status`) and gets an empty row; nothing
     is copied or counted for it, and the other children are made."""
     r = _C().kv_fork(kv_cache, block_table, seq_lens, parents, fresh, ref)
-    _count(2 if parents.shape[0] else 0)
+    _count()
     return r
 
 

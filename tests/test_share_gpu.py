@@ -804,3 +804,29 @@ def test_kv_free_and_compact_pass_over_bad_ids(bad):
     assert torch.equal(got[0], moved) and torch.equal(got[1], used)
     for a, w in zip((cache, table, n, count), want):
         assert torch.equal(a, w)
+
+
+@pytest.mark.parametrize("layers,parents", [(1, [0] * 3000), (33000, [0, 1, -1, 1]), (70, [1] * 40)])
+def test_kv_fork_many_children_and_layers(layers, parents):
+    """Children by the thousand, and more copy steps of a child than CTAs copy."""
+    cache, table, n, count, free = page_state("tiny", [37, 21], spare=len(parents), layers=layers)
+    check_fork((cache, table, n, i32(parents), i32(free[:len(parents)]), count))
+
+
+def test_kv_fork_of_one_fresh_page_by_many_children():
+    """One of the children is made, whole, whichever it is; a page that somebody holds is claimed by none."""
+    cache, table, n, count, free = page_state("int8", [23 + 16 * (i % 3) for i in range(40)], layers=20)
+    held = int(table[7, 0])
+    fresh = torch.full((40,), free[0], dtype=torch.int32, device="cuda")
+    fresh[30:] = held
+    for _ in range(3):
+        want, count_want = cache.clone(), count.clone()
+        t, lens = ops.kv_fork(cache, table, n, i32(list(range(40))), fresh, count)
+        assert took_bits() == BAD
+        made = (lens > 0).nonzero()[:, 0].tolist()
+        assert len(made) == 1 and made[0] < 30
+        parents = i32([c if c in made else -1 for c in range(40)])
+        wt, wl = ref.kv_fork(want, table, n, parents, fresh, count_want)
+        assert torch.equal(t, wt) and torch.equal(lens, wl) and torch.equal(cache, want)
+        assert torch.equal(count, count_want)
+        ops.kv_free(t, lens, i32(made), count)
