@@ -16,6 +16,7 @@ import json
 import math
 import os
 import statistics
+import time
 
 import torch
 
@@ -427,9 +428,14 @@ def main():
             lens = torch.full((B,), prefix + tail, dtype=torch.int32, device=dev)
             q = torch.randn(B, nq, hd, device=dev, dtype=torch.bfloat16)
             out = torch.empty_like(q)
-            plan = ops.shared_prefix_plan([members] * groups, [prefix] * groups, num_q_heads=nq, num_kv_heads=nkv,
-                                          head_dim=hd, max_seq_len=prefix + tail, device=dev)
             ex = {"groups": groups, "members": members, "prefix": prefix, "own": tail}
+            host = []
+            for _ in range(5):  # made on the host, kept until a member is added
+                t0 = time.perf_counter()
+                plan = ops.shared_prefix_plan([members] * groups, [prefix] * groups, num_q_heads=nq, num_kv_heads=nkv,
+                                              head_dim=hd, max_seq_len=prefix + tail, device=dev)
+                host.append(time.perf_counter() - t0)
+            report("shared_prefix_plan", statistics.median(host) * 1e3, extra=ex)
             ms = timeit(lambda i=0: ops.shared_prefix_attention(q, kv, 0, table, lens, out, plan=plan,
                                                                 scale=hd ** -0.5))
             report("shared_prefix_attention", ms, 4.0 * B * (prefix + tail) * nq * hd, nb * 2 * nkv * 16 * hd * 2, ex)

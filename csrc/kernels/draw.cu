@@ -21,8 +21,9 @@
 // and equal values are counted off in vocabulary order.  Histograms are reduced over the cluster through distributed
 // shared memory.  The draw walks vocabulary order: sums of 256 tokens, a scan, and one warp for the chunk that
 // holds u Z.
-// Measured with 128,256 bf16 logits a row: one row 9 us plain, 16 top-k, 30 top-p (cluster barriers, a sort); 256 rows
-// 69, 95 and 228 us, bound by instructions (40, 60 and 120 a token; reading the row is 10 us).
+// Measured with 128,256 bf16 logits a row (normal, deviation 3): one row 9 us plain, 16 top-k 50, 29 top-p 0.9 (cluster
+// barriers, a sort); 256 rows 69, 95 and 227 us, bound by instructions (40, 60 and 120 a token; reading the row is
+// 10 us).  Two CTAs per SM leave 64 registers a thread: 44 bytes of spills for bf16, 20 for fp32.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cooperative_groups.h>

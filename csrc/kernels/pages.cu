@@ -13,10 +13,11 @@
 //
 // All three are bound by the bytes of the pages they copy (each read once and written once), and at small sizes by
 // launches: fork and free are one launch, compact is two (a one-CTA plan over a bitmap of ref, then the copies).
-// Copies run in chunks of 16 or 32 KB per CTA, all loads of a chunk in flight before its first store: 8 CTAs per SM
-// keep 128 KB or more in flight, which covers the bandwidth-latency product (44 GB/s per SM x ~2 us).
-// Measured: a pool of 18,000 pages compacts at 6.5 TB/s (read + write) after a plan of 8 to 11 us; a fork of 4 children takes
-// 3.7 us in a graph, of 128 children over 8 layers 11.9 us.
+// Copies run in chunks of 16 or 32 KB per CTA that end with the page, all loads of a chunk in flight before its first
+// store.  With whole chunks an SM has 96 KB (fork: 6 CTAs, 40 registers a thread) or 128 KB (compact: 4 CTAs, 60
+// registers) in flight, against a bandwidth-latency product of 88 KB (44 GB/s per SM x ~2 us).
+// Measured: a pool of 18,000 pages compacts at 6.5 TB/s (read + write) after a plan of 8 to 11 us; a fork of 4 children
+// over 16 layers and a reset of the counts take 5.1 us in a graph, of 128 children over 8 layers of int8 pages 12.0.
 //
 // An id outside its range sets kStatusBadArgument and its access is skipped, in every build.
 //
@@ -36,8 +37,8 @@ namespace pages {
 
 constexpr int kPage = 16;
 constexpr int kThreads = 256;
-// 16-byte loads in flight per thread.  Eight where the copies last (645 MB compacted in 99 us, 106 with four), four where
-// a fork's CTAs are few (34 MB in 11.9 us, 12.5 with eight).
+// 16-byte loads in flight per thread.  Eight where the copies last (645 MB compacted in 99 us, 106 with four), four in
+// a fork, whose CTAs hold them while they ask for their page (34 MB in 12.0 us, 14.5 with eight and four CTAs per SM).
 constexpr int kForkVec = 4, kMoveVec = 8;
 template <int kVec>
 constexpr int kChunk = kThreads * kVec * 16;  // bytes of one copy step of a CTA
@@ -482,7 +483,7 @@ std::tuple<torch::Tensor, torch::Tensor> kv_compact(torch::Tensor& kv_cache, tor
     C10_CUDA_CHECK(cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxPages / 8));
   plan_kernel<<<1, kPlanThreads, smem, stream>>>(a);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  // no more copy CTAs than there can be chunks, and at most 8 per SM
+  // no more copy CTAs than there can be chunks, and at most 8 per SM (4 at a time; each goes on to further chunks)
   const long most = std::max<long>(1, (long)(NB / 2) * a.L * a.chunks);
   const int copiers = int(std::min<long>(most, 8L * num_sms(kv_cache.get_device())));
   cudaLaunchConfig_t cfg = {};  // a dependent launch: its CTAs are there when the plan is done

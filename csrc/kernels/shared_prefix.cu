@@ -13,9 +13,10 @@
 // whose prefix is work for the tensor cores: both side by side on two streams, and a third kernel adds the parts.
 //
 // Bound by: few sequences, a chain of dependent loads (10 us with 4 sequences behind 512 tokens); many, the prefix's
-// softmax (50 us for 35 GFLOP) beside the suffixes' pages (62 us for 268 MB of uneven lengths): 106 us together.  The
-// decode kernel that reads every sequence's whole table takes 828 us for 256 sequences behind 8,192 tokens where this
-// takes 93, and 63 us for 32 behind 4,096 where this takes 25.
+// softmax (50 us for 35 GFLOP) beside the suffixes' pages (63 us for 268 MB of 1 to 511 tokens each): 107 us together
+// for 256 sequences behind 8,192 tokens, 93 where each has 256 of its own; the decode kernel that reads every sequence's
+// whole table takes 826.  32 sequences behind 4,096 tokens, 128 of their own: 25 us, decode kernel 63.  (32 / 8 heads of
+// 128, captured.)
 //
 // Slots behind a sequence's last token may hold anything (NaN too): scores there are replaced, and V rows there are
 // zeroed in shared memory.  A block id outside the cache sets kStatusBadArgument and page 0 is read instead.
