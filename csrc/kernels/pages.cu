@@ -81,11 +81,12 @@ struct ForkArgs {
   int* status;
 };
 
-// A fresh page is claimed before a byte of it is written.  Every CTA of child c asks for the claim: the count of a free page
-// goes from 0 to a tag of c, and for the time of the launch it is kClaim | c << kClaimBits | CTAs of c that have asked; the
-// last of them makes it 1.  It leaves 0 once and for good, so all CTAs of a child get one answer, and a page that somebody
-// holds, or that another child has claimed, is left as it is.  (A first kernel for the claims and a dependent one for the
-// copies took 14.6 us where this takes 12.0: 128 children over 8 layers of int8 pages and a reset of the counts, in a graph.)
+// A fresh page is claimed before a byte of it is written.  Every CTA of child c asks for the claim: the count of a free
+// page goes from 0 to a tag of c, and for the time of the launch it is kClaim | c << kClaimBits | CTAs of c that have
+// asked; the last of them makes it 1.  It leaves 0 once and for good, so all CTAs of a child get one answer, and a page
+// that somebody holds, or that another child has claimed, is left as it is.  (A first kernel for the claims and a
+// dependent one for the copies took 14.6 us where this takes 12.0: 128 children over 8 layers of int8 pages and a reset
+// of the counts, in a graph.)
 constexpr int kClaimBits = 15, kForkCtas = (1 << kClaimBits) - 1;
 constexpr int kForkPerSm = 6;  // CTAs per SM, 40 registers a thread
 constexpr int64_t kMaxChildren = 65535;
